@@ -299,6 +299,51 @@ int olmo355_attn_decode_fused(const void* qkv, const void* qw, const void* kw, c
 int olmo355_rope_advance(int32_t* pos, int delta, const float* sin_tab, const float* cos_tab, float* rope_now, int hd,
                          int n_pos, void* stream);
 
+/* ---- the cache in 8 bits ------------------------------------------------------------------------
+ * A cached row (one token, one kv head) is hd signed codes and one fp32 scale: scale = max(max |x| / 127, FLT_MIN),
+ * code = rint(x / scale), x ~ code * scale.  A row that holds an infinity or a NaN gets the scale NaN (it reads back as
+ * NaN; a masked key of that kind does not reach an output).  kq, vq: int8 [B, Hkv, Lmax, hd]; kscale, vscale: float
+ * [B, Hkv, Lmax]; keys rotated, as in the unquantised cache.  hd 32, 64 or 128.  Activations, tables, codes and outputs
+ * 16-byte aligned (O355_EINVAL otherwise).  No counterpart in the reference, whose cache holds the activation type
+ * (olmo/model.py:615-620). */
+/* olmo355_qknorm_rope_kvwrite into that form: q_out [B*T, H*hd] in the activation type, codes and scales of rows
+ * past_len + t.  fp32 from qkv to q's one rounding and to the codes (no rounding between norm, rotation and
+ * quantisation).  kcache / vcache: both NULL, or [B, Hkv, Lmax, hd] in the activation type, which receive the same
+ * rows unquantised (for a prefill's own attention).  past_len_dev needs T == 1; a position outside the cache or the tables
+ * then writes nothing.  H*hd up to 16384. */
+int olmo355_qknorm_rope_kvwrite_q8(const void* qkv, const void* qw, const void* kw, const float* sin_tab,
+                                   const float* cos_tab, void* q_out, int8_t* kq, int8_t* vq, float* kscale, float* vscale,
+                                   void* kcache, void* vcache, int B, int T, int H, int Hkv, int hd, int Lmax, int n_pos,
+                                   int past_len, const int32_t* past_len_dev, float eps, int dtype, void* stream);
+/* Rows start .. start + n - 1 of every (sequence, kv head) back as values: code * scale, one rounding to `dtype`, into
+ * rows out_start .. of kout / vout [B, Hkv, Lout, hd]. */
+int olmo355_kv_read_q8(const int8_t* kq, const int8_t* vq, const float* kscale, const float* vscale, void* kout, void* vout,
+                       int B, int Hkv, int hd, int Lmax, int start, int n, int Lout, int out_start, int dtype, void* stream);
+/* olmo355_attn_decode over that form: one query per sequence, scores (q . codes) * kscale / sqrt(hd) + bias, masked keys
+ * (bias <= -1e30) as there.  ws: olmo355_attn_decode_q8_workspace_bytes(...) bytes, 16-byte aligned (0: ws may be NULL);
+ * nothing in it outlives the call, so it needs no clearing and serves any launch of at most its size that is ordered
+ * with the others on one stream. */
+int64_t olmo355_attn_decode_q8_workspace_bytes(int B, int H, int Hkv, int hd, int n_keys_max);
+int olmo355_attn_decode_q8(const void* q, const int8_t* kq, const int8_t* vq, const float* kscale, const float* vscale,
+                           const float* key_bias, void* out, void* ws, int64_t ws_bytes, int B, int H, int Hkv, int hd,
+                           int Lmax, int past_len, const int32_t* past_len_dev, int n_keys_max, int bias_stride, int dtype,
+                           void* stream);
+
+/* ---- attention of a batch that shares a prefix -----------------------------------------------------
+ * q [B*T, H*hd]; kprefix / vprefix [Hkv, Pmax, hd]: rows 0 .. prefix_len - 1 are seen by every query of every sequence;
+ * kcache / vcache [B, Hkv, Lmax, hd]: the sequences' own rows, of which query t sees 0 .. past_len + t.  Equal to
+ * olmo355_attn_prefill / olmo355_attn_decode over a cache that begins with a copy of the prefix, read once for all sequences.
+ * key_bias (may be NULL): fp32 [B, bias_stride] for the own rows; a masked one (<= -1e30) weighs nothing, whatever it
+ * holds (the prefix is never masked, so no query is left without a key).  prefix_len >= 1, n_keys_max >= T bounds the own
+ * rows for the launch grid (past_len + T <= n_keys_max <= Lmax); past_len_dev needs T == 1.  hd 32, 64 or 128; q, caches
+ * and out 16-byte aligned.  ws as for olmo355_attn_decode_q8. */
+int64_t olmo355_attn_shared_prefix_workspace_bytes(int B, int T, int H, int Hkv, int hd, int prefix_len, int n_keys_max,
+                                                   int dtype);
+int olmo355_attn_shared_prefix(const void* q, const void* kprefix, const void* vprefix, const void* kcache,
+                               const void* vcache, const float* key_bias, void* out, void* ws, int64_t ws_bytes, int B, int T,
+                               int H, int Hkv, int hd, int prefix_len, int Pmax, int Lmax, int past_len,
+                               const int32_t* past_len_dev, int n_keys_max, int bias_stride, int dtype, void* stream);
+
 /* ---- MLP activation: SwiGLU.forward (olmo/model.py:365-368) --------------------------------
  * x [rows, 2h]: first half "up", second half "gate"; out [rows, h] = silu(gate) * up. */
 int olmo355_swiglu(const void* x, void* out, int rows, int h, int dtype, void* stream);

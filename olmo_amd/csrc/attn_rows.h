@@ -1,0 +1,409 @@
+// Attention of a few query rows over a run of cached keys, on the matrix cores, straight from memory: the body that
+// the decode attention over the 8-bit cache (kvq8.hip) and the attention under a shared prefix (prefix.hip) have in common.
+//
+//   x_j = (q . k_j) / sqrt(hd) + bias_j,   p_j = 2^(x_j log2 e - m),   out = sum p_j v_j / sum p_j
+//
+// One pass with a running maximum m and denominator per row (fp32).  A wave takes 32 keys at a time and up to 16 * RT
+// rows; the four waves of a workgroup take every fourth run of 32 and merge at the end through LDS.
+//
+// Operands come from memory in the shape the matrix instruction wants, without a trip through LDS:
+//   S^T = K . Q^T    lane (key = l & 15, kq = l >> 4) holds 8 channels of its key: pieces of a cache row
+//   O^T = V^T . P^T  the operand wants 8 *keys* of one channel per lane.  A lane loads, for its 8 keys, the VC = hd / 16
+//                    channels (l & 15) * VC ..; channel tile j of the product then takes element j of each of the 8 rows
+//                    (a permuted numbering of the output channels, undone when the result is written).
+//   The 8 keys of lane group kq are 4 kq .. + 3 and 16 + 4 kq .. + 3 of the 32: where the accumulators of S^T already
+//   sit, so the probabilities go from accumulators to the second product inside the lane.
+#pragma once
+#include "common.h"
+
+namespace {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
+typedef f32x4 f32x4_a4 __attribute__((aligned(4)));
+
+constexpr float kRowsMaskThreshold = -1e30f;  // bias entries at or below: the key is masked
+constexpr float kRowsLazyMax = 8.f;           // log2 units the running maximum may lag behind (probabilities stay below 2^8)
+constexpr float kLog2e = 1.4426950408889634f;
+
+// eight consecutive elements along k of a matrix operand, and the 16 x 16 x 32 product of two such fragments
+template <int DT> struct Frag8;
+template <> struct Frag8<O355_BF16> {
+  typedef bf16x8 T;
+  static __device__ __forceinline__ T ld(const void* p) { return *reinterpret_cast<const bf16x8*>(p); }
+  static __device__ __forceinline__ T pack(const float (&f)[8]) {
+    const u32x4 w = {pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])};
+    return __builtin_bit_cast(bf16x8, w);
+  }
+  static __device__ __forceinline__ f32x4 mma(T a, T b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Frag8<O355_F16> {
+  typedef f16x8 T;
+  static __device__ __forceinline__ T ld(const void* p) { return *reinterpret_cast<const f16x8*>(p); }
+  static __device__ __forceinline__ T pack(const float (&f)[8]) {
+    const u32x4 w = {pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]), pack_f16x2(f[4], f[5]), pack_f16x2(f[6], f[7])};
+    return __builtin_bit_cast(f16x8, w);
+  }
+  static __device__ __forceinline__ f32x4 mma(T a, T b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Frag8<O355_F32> {  // eight 16 x 16 x 4 products: full fp32
+  struct T { float f[8]; };
+  static __device__ __forceinline__ T ld(const void* p) {
+    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+    return T{{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}};
+  }
+  static __device__ __forceinline__ T pack(const float (&f)[8]) { return T{{f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7]}}; }
+  static __device__ __forceinline__ f32x4 mma(const T& a, const T& b, f32x4 c) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.f[i], b.f[i], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// N words from 4 N-byte aligned memory (N = 1, 2, 4, 8)
+template <int N>
+__device__ __forceinline__ void ld_words(const void* p, uint32_t (&w)[N]) {
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (N == 2) {
+    const u32x2 v = *reinterpret_cast<const u32x2*>(p);
+    w[0] = v[0], w[1] = v[1];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const u32x4 v = reinterpret_cast<const u32x4*>(p)[i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[4 * i + e] = v[e];
+    }
+  }
+}
+
+// ---- the 32 keys of one step as they come from memory -------------------------------------------------------
+// K / V in the activation type.  kb, vb: the step's first row; row[i]: the lane's rows within the step (already
+// clamped to the last key): row_k[2] for the two key tiles, row_v[8] for its 8 keys.
+template <int DT, int HD>
+struct RawKeys {
+  static constexpr bool SCALED = false;
+  static constexpr int PV = DT;  // type of the second product
+  static constexpr int ES = DT == O355_F32 ? 4 : 2, STEPS = HD / 32, VC = HD / 16, VW = VC * ES / 4;
+  typename Frag8<DT>::T k[2][STEPS];
+  uint32_t v[8][VW];
+  static __device__ __forceinline__ int q_elem(int s, int kq) { return 32 * s + 8 * kq; }
+  __device__ __forceinline__ void load(const unsigned char* kb, const unsigned char* vb, const int (&row_k)[2], const int (&row_v)[8],
+                                       int col, int kq) {
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) k[kt][s] = Frag8<DT>::ld(kb + (uint32_t)(row_k[kt] * (HD * ES) + (32 * s + 8 * kq) * ES));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ld_words<VW>(vb + (uint32_t)(row_v[e] * (HD * ES) + col * (VC * ES)), v[e]);
+  }
+  __device__ __forceinline__ typename Frag8<DT>::T kfrag(int kt, int s) const { return k[kt][s]; }
+  __device__ __forceinline__ typename Frag8<DT>::T vfrag(int j) const {
+    if constexpr (DT == O355_F32) {
+      typename Frag8<DT>::T r;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r.f[e] = __uint_as_float(v[e][j]);
+      return r;
+    } else {
+      u32x4 w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)  // half j & 1 of word j / 2 of two neighbouring keys
+        w[i] = __builtin_amdgcn_perm(v[2 * i + 1][j >> 1], v[2 * i][j >> 1], (j & 1) ? 0x07060302u : 0x05040100u);
+      return __builtin_bit_cast(typename Frag8<DT>::T, w);
+    }
+  }
+  __device__ __forceinline__ void drop(int e) {  // key e of the lane weighs nothing, whatever its values hold
+#pragma unroll
+    for (int i = 0; i < VW; ++i) v[e][i] = 0;
+  }
+};
+
+// K / V as 8-bit codes.  A 16-byte load holds two steps' worth of a key: its channels 64 i + 16 kq .. + 15.
+template <int DT, int HD>
+struct Q8Keys {
+  static constexpr bool SCALED = true;
+  // The value codes are multiplied with p * scale rounded to bf16 (relative 2^-8 per term, in a sum over keys) for both
+  // 16-bit types: p * scale has no bound that would keep it inside fp16's range.  fp32 activations stay in fp32.
+  static constexpr int PV = DT == O355_F32 ? O355_F32 : O355_BF16;
+  static constexpr int STEPS = HD / 32, VC = HD / 16, KW = HD / 16;  // KW: words of a key per lane
+  uint32_t k[2][KW];
+  u32x2 v[8];  // VC codes: 8, 4 or 2 of the bytes
+  static __device__ __forceinline__ int q_elem(int s, int kq) { return HD == 32 ? 8 * kq : 64 * (s >> 1) + 16 * kq + 8 * (s & 1); }
+  __device__ __forceinline__ void load(const unsigned char* kb, const unsigned char* vb, const int (&row_k)[2], const int (&row_v)[8],
+                                       int col, int kq) {
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      if constexpr (HD == 32) {
+        ld_words<2>(kb + (uint32_t)(row_k[kt] * HD + 8 * kq), k[kt]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < HD / 64; ++i) {
+          const u32x4 w = *reinterpret_cast<const u32x4*>(kb + (uint32_t)(row_k[kt] * HD + 64 * i + 16 * kq));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) k[kt][4 * i + e] = w[e];
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned char* p = vb + (uint32_t)(row_v[e] * HD + col * VC);
+      if constexpr (VC == 8) v[e] = *reinterpret_cast<const u32x2*>(p);
+      else if constexpr (VC == 4) v[e] = u32x2{*reinterpret_cast<const uint32_t*>(p), 0u};
+      else v[e] = u32x2{(uint32_t)*reinterpret_cast<const uint16_t*>(p), 0u};
+    }
+  }
+  static __device__ __forceinline__ float code(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
+  __device__ __forceinline__ typename Frag8<DT>::T kfrag(int kt, int s) const {
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = code(k[kt][2 * s + (e >> 2)], e & 3);
+    return Frag8<DT>::pack(f);  // integers up to 127: exact in every type
+  }
+  __device__ __forceinline__ typename Frag8<PV>::T vfrag(int j) const {
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = code(v[e][j >> 2], j & 3);
+    return Frag8<PV>::pack(f);
+  }
+  __device__ __forceinline__ void drop(int) {}  // codes are finite; the caller drops the key's scale
+};
+
+// ---- one workgroup: rows x keys -> merged (m, l, o) -----------------------------------------------------------
+struct RowsIn {
+  const unsigned char* q;  // the activation rows [token][H][HD]
+  int tok0;                // row r belongs to token tok0 + r / G, head head0 + r % G
+  int G, H, head0;
+  int r0, nrows;           // rows r0 .. nrows - 1 are this workgroup's (at most 16 * RT of them are taken)
+  const unsigned char *k, *v;   // this kv head's keys and values, row 0
+  const float *ks, *vs;         // scales of the 8-bit form
+  const float* bias;            // per key, or NULL
+  int step_lo, step_hi;         // runs of 32 keys
+  int keys;                     // keys in all (rows past them are not read)
+  int past;                     // causal: row r sees keys <= past + r / G; -1: all keys
+};
+
+template <int HD>
+struct RowsLds {
+  static constexpr int PITCH = HD + 4;
+  float m[4][64], l[4][64];
+  float o[4][16][PITCH];
+};
+
+// What a row's masked keys count: KEEP_MASKED: a masked key keeps the type's lowest value as its score (so a row of nothing
+// but masked keys averages them, as the decode attention does); otherwise it weighs nothing.
+// emit(row, channel, VC values of o, m, l): called by 16 threads per row, once for every row of the workgroup.
+template <int DT, int HD, int RT, bool KEEP_MASKED, class Keys, class Emit>
+__device__ __forceinline__ void attend_rows(const RowsIn& in, RowsLds<HD>& lds, Emit emit) {
+  typedef Frag8<DT> FQ;
+  typedef Frag8<Keys::PV> FP;
+  constexpr int STEPS = HD / 32, VC = HD / 16, ES = DT == O355_F32 ? 4 : 2;
+  constexpr int KROW = Keys::SCALED ? HD : HD * ES;  // bytes of a key row
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, kq = lane >> 4;
+  const float c2 = kLog2e / sqrtf((float)HD);  // scores in the log2 domain
+  const float lowest = Act<DT>::lowest();
+
+  typename FQ::T qf[RT][STEPS];
+  int sees[RT];  // last key visible to the row
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = min(in.r0 + 16 * rt + col, in.nrows - 1);
+    const int t = r / in.G;
+    sees[rt] = in.past < 0 ? in.keys - 1 : in.past + t;
+    const unsigned char* src = in.q + (((int64_t)(in.tok0 + t) * in.H + in.head0 + (r - t * in.G)) * HD) * ES;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) qf[rt][s] = FQ::ld(src + Keys::q_elem(s, kq) * ES);
+  }
+  f32x4 o[RT][VC];
+  float m[RT], l[RT];  // l: this lane's share (8 of 32 keys)
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    m[rt] = -INFINITY, l[rt] = 0.f;
+#pragma unroll
+    for (int j = 0; j < VC; ++j) o[rt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const bool causal = in.past >= 0;
+
+  for (int step = in.step_lo + wave; step < in.step_hi; step += 4) {
+    const int k0 = step * 32, left = in.keys - 1 - k0;  // left >= 0: the last row of the step that exists
+    int row_k[2] = {col, 16 + col}, row_v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) row_v[e] = 4 * kq + (e & 3) + 16 * (e >> 2);
+    int row_s[2] = {4 * kq, 16 + 4 * kq};  // first of four scale / bias entries
+    const bool tail = left < 31;
+    if (tail) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) row_k[i] = min(row_k[i], left);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) row_v[e] = min(row_v[e], left);
+    }
+    Keys kv;
+    kv.load(in.k + (int64_t)k0 * KROW, in.v + (int64_t)k0 * KROW, row_k, row_v, col, kq);
+    float sk[8], sv[8], bs[8];
+    auto ld8 = [&](const float* p, float (&f)[8]) {
+      if (tail) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = p[row_v[e]];
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const f32x4 w = *reinterpret_cast<const f32x4_a4*>(p + row_s[h]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) f[4 * h + e] = w[e];
+        }
+      }
+    };
+    if constexpr (Keys::SCALED) ld8(in.ks + k0, sk), ld8(in.vs + k0, sv);
+    if (in.bias) ld8(in.bias + k0, bs);
+
+    // ---- S^T = K . Q^T
+    f32x4 s[RT][2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int st = 0; st < STEPS; ++st) {
+        const auto kf = kv.kfrag(kt, st);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s[rt][kt] = FQ::mma(kf, qf[rt][st], st == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[rt][kt]);
+      }
+    if (in.bias && !KEEP_MASKED) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (bs[e] <= kRowsMaskThreshold) kv.drop(e);
+    }
+    // ---- running maximum, probabilities
+    typename FP::T pf[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float x[8], tmax = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float v = s[rt][e >> 2][e & 3] * c2;
+        if constexpr (Keys::SCALED) v *= sk[e];
+        if (in.bias) {
+          v = __builtin_fmaf(bs[e], kLog2e, v);
+          v = bs[e] <= kRowsMaskThreshold ? (KEEP_MASKED ? lowest : -INFINITY) : v;
+        }
+        const int key = 4 * kq + (e & 3) + 16 * (e >> 2);
+        if (tail || causal) v = k0 + key > min(sees[rt], in.keys - 1) ? -INFINITY : v;
+        x[e] = v;
+        tmax = fmaxf(tmax, v);
+      }
+      // The reference maximum moves only when some row's new maximum is more than kRowsLazyMax above it.
+      if (__builtin_amdgcn_ballot_w64(tmax > m[rt] + kRowsLazyMax) != 0) {
+        tmax = combine_xor32(combine_xor16(tmax, MaxOp{}), MaxOp{});
+        const float mn = tmax > m[rt] + kRowsLazyMax ? tmax : m[rt];
+        const float alpha = mn == m[rt] ? 1.f : __builtin_amdgcn_exp2f(m[rt] - mn);
+        l[rt] *= alpha;
+#pragma unroll
+        for (int j = 0; j < VC; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[rt][j][r] = alpha == 0.f ? 0.f : o[rt][j][r] * alpha;  // see `weigh`
+        m[rt] = mn;
+      }
+      const float mref = m[rt] == -INFINITY ? 0.f : m[rt];  // a row that has seen no key yet
+      float p[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(x[e] - mref);
+        l[rt] += p[e];
+        if constexpr (Keys::SCALED) p[e] = p[e] == 0.f ? 0.f : p[e] * sv[e];  // the scale of a key that weighs nothing may be NaN
+      }
+      pf[rt] = FP::pack(p);
+    }
+    // ---- O^T += V^T . P^T
+#pragma unroll
+    for (int j = 0; j < VC; ++j) {
+      const auto vf = kv.vfrag(j);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) o[rt][j] = FP::mma(vf, pf[rt], o[rt][j]);
+    }
+  }
+
+  // ---- the four waves' results into one
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    l[rt] = combine_xor32(combine_xor16(l[rt], AddOp{}), AddOp{});
+    if (kq == 0) lds.m[wave][16 * rt + col] = m[rt], lds.l[wave][16 * rt + col] = l[rt];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    float mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, lds.m[w][16 * rt + col]);
+    // weigh: what a wave gathered under a maximum that turns out to weigh nothing is left out, not multiplied by zero: it
+    // may be the mean of masked keys' values, which are not looked at once the row has a key that is not masked
+    const float alpha = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rt] - mm);
+    if (in.r0 + 16 * rt + col < in.nrows) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < VC; ++j) lds.o[wave][col][(4 * kq + r) * VC + j] = alpha == 0.f ? 0.f : o[rt][j][r] * alpha;
+    }
+    __syncthreads();
+    const int rr = tid >> 4, c = (tid & 15) * VC, row = in.r0 + 16 * rt + rr;
+    if (row < in.nrows) {
+      float ov[VC], mrow = -INFINITY, lrow = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mrow = fmaxf(mrow, lds.m[w][16 * rt + rr]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float mw = lds.m[w][16 * rt + rr], lw = lds.l[w][16 * rt + rr];
+        lrow += mw == -INFINITY ? lw : lw * __builtin_amdgcn_exp2f(mw - mrow);  // lw is 0 there, or NaN from a NaN score
+      }
+#pragma unroll
+      for (int j = 0; j < VC; ++j) ov[j] = (lds.o[0][rr][c + j] + lds.o[1][rr][c + j]) + (lds.o[2][rr][c + j] + lds.o[3][rr][c + j]);
+      emit(row, c, ov, mrow, lrow);
+    }
+    if (rt + 1 < RT) __syncthreads();
+  }
+}
+
+// VC consecutive values of an output row
+template <int DT, int VC>
+__device__ __forceinline__ void st_row(void* out, int64_t elem, const float (&f)[VC]) {
+  if constexpr (DT == O355_F32) {
+#pragma unroll
+    for (int i = 0; i < VC; i += 2) *reinterpret_cast<u32x2*>((float*)out + elem + i) = u32x2{__float_as_uint(f[i]), __float_as_uint(f[i + 1])};
+  } else {
+#pragma unroll
+    for (int i = 0; i < VC; i += 2)
+      *reinterpret_cast<uint32_t*>((uint16_t*)out + elem + i) = DT == O355_BF16 ? pack_bf16x2(f[i], f[i + 1]) : pack_f16x2(f[i], f[i + 1]);
+  }
+}
+
+// Partial results of rows whose keys several workgroups share: o unnormalised [part][rows][HD], then (m, l) [part][rows].
+__host__ __device__ __forceinline__ int64_t rows_parts_floats(int64_t rows, int hd, int parts) { return rows * parts * (hd + 2); }
+
+template <int DT, int HD>
+__global__ __launch_bounds__(256) void rows_combine_kernel(const float* __restrict__ ws, void* __restrict__ out, int64_t rows, int parts) {
+  constexpr int VC = HD / 16;
+  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int c = (threadIdx.x & 15) * VC;
+  if (row >= rows) return;
+  const float* ml = ws + rows * parts * HD;
+  float mm = -INFINITY, l = 0.f, o[VC];
+  for (int i = 0; i < parts; ++i) mm = fmaxf(mm, ml[(i * rows + row) * 2]);
+#pragma unroll
+  for (int j = 0; j < VC; ++j) o[j] = 0.f;
+  for (int i = 0; i < parts; ++i) {
+    const float mi = ml[(i * rows + row) * 2], li = ml[(i * rows + row) * 2 + 1];
+    if (mi == -INFINITY) {
+      l += li;  // 0, or NaN from a NaN score
+      continue;
+    }
+    const float w = __builtin_amdgcn_exp2f(mi - mm);
+    l += li * w;
+    if (w == 0.f) continue;
+#pragma unroll
+    for (int j = 0; j < VC; ++j) o[j] += w * ws[(i * rows + row) * HD + c + j];
+  }
+  const float inv = 1.f / l;
+#pragma unroll
+  for (int j = 0; j < VC; ++j) o[j] *= inv;
+  st_row<DT, VC>(out, row * HD + c, o);
+}
+
+}  // namespace

@@ -1,0 +1,338 @@
+// The key/value cache in 8 bits: written together with the QK-norm and the rotation, read back, and attended to by the
+// one new token of a decode step.
+//
+// A cached row (one token, one kv head, hd channels) is hd signed codes and one fp32 scale:
+//   scale = max(max |x| / 127, FLT_MIN),  code = rint(x / scale) in -127 .. 127,  x ~ code * scale
+// (the lower bound keeps the reciprocal finite; a row of zeros has codes 0).  The row's own maximum makes the error at most
+// half a step of max / 127 whatever the row's size.  A row that holds an infinity or a NaN gets the scale NaN and codes 0:
+// it reads back as NaN, and attention gives NaN unless the key is masked.
+// Layout: codes int8 [B, Hkv, Lmax, hd], scales fp32 [B, Hkv, Lmax], keys rotated as in the unquantised cache.
+#include "attn_rows.h"
+
+namespace {
+
+// eight activations as floats, and back (16 bytes of a 16-bit type, 32 of fp32)
+template <int DT>
+__device__ __forceinline__ void ld8f(const void* p, int64_t e, float (&f)[8]) {
+  if constexpr (DT == O355_F32) {
+    const f32x4 a = reinterpret_cast<const f32x4*>((const float*)p + e)[0], b = reinterpret_cast<const f32x4*>((const float*)p + e)[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = a[i], f[4 + i] = b[i];
+  } else {
+    const u32x4 w = *reinterpret_cast<const u32x4*>((const uint16_t*)p + e);
+    if constexpr (DT == O355_BF16) {
+      unpack8(w, f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f16x2 h = __builtin_bit_cast(f16x2, (uint32_t)w[i]);
+        f[2 * i] = (float)h[0], f[2 * i + 1] = (float)h[1];
+      }
+    }
+  }
+}
+template <int DT>
+__device__ __forceinline__ void st8f(void* p, int64_t e, const float (&f)[8]) {
+  if constexpr (DT == O355_F32) {
+    reinterpret_cast<f32x4*>((float*)p + e)[0] = f32x4{f[0], f[1], f[2], f[3]};
+    reinterpret_cast<f32x4*>((float*)p + e)[1] = f32x4{f[4], f[5], f[6], f[7]};
+  } else if constexpr (DT == O355_BF16) {
+    *reinterpret_cast<u32x4*>((uint16_t*)p + e) =
+        u32x4{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])};
+  } else {
+    *reinterpret_cast<u32x4*>((uint16_t*)p + e) =
+        u32x4{pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]), pack_f16x2(f[4], f[5]), pack_f16x2(f[6], f[7])};
+  }
+}
+
+// ---- write ----------------------------------------------------------------------------------------------------
+// Grid (token row, part): part 0 normalises and rotates q, part 1 k, part 2 takes v: the sum of squares of q and of k are
+// over the whole width (olmo/model.py:603-605), so a workgroup needs one of them and reads nothing twice.  A thread owns
+// channels j .. j + 7 of the first half of a head and the 8 they rotate with; hd / 16 neighbouring lanes hold a head, whose
+// maximum is a few register exchanges.  fp32 from the input to the code (q: to its one rounding).
+template <int DT, int HD, int CPT>
+__global__ __launch_bounds__(256) void kv_write_q8_kernel(const void* __restrict__ qkv, const void* __restrict__ qw,
+                                                          const void* __restrict__ kw, const float* __restrict__ sin_t,
+                                                          const float* __restrict__ cos_t, void* __restrict__ q_out,
+                                                          int8_t* __restrict__ kq, int8_t* __restrict__ vq, float* __restrict__ ks,
+                                                          float* __restrict__ vs, void* __restrict__ kc, void* __restrict__ vc, int T,
+                                                          int H, int Hkv, int Lmax, int n_pos, int past_len,
+                                                          const int32_t* __restrict__ past_dev, float eps) {
+  constexpr int CPH = HD / 16, HALF = HD / 2;
+  __shared__ float red[16];
+  const int part = blockIdx.y;
+  const int64_t row = blockIdx.x;
+  const int b = (int)(row / T), t = (int)(row - (int64_t)b * T);
+  const int dq = H * HD, dk = Hkv * HD;
+  const int pos = (past_dev ? *past_dev : past_len) + t;
+  if (pos < 0 || pos >= Lmax || pos >= n_pos) return;  // a device-side position outside the cache: write nothing
+  const int heads = part == 0 ? H : Hkv, n = heads * CPH;
+  const int64_t in = row * (dq + 2 * dk) + (part == 0 ? 0 : part == 1 ? dq : dq + dk);
+  const void* w = part == 0 ? qw : part == 1 ? kw : nullptr;
+  float x1[CPT][8], x2[CPT][8];
+#pragma unroll
+  for (int i = 0; i < CPT; ++i) {
+    const int c = threadIdx.x + i * 256;
+    if (c < n) {
+      const int64_t e = in + (c / CPH) * HD + (c % CPH) * 8;
+      ld8f<DT>(qkv, e, x1[i]);
+      ld8f<DT>(qkv, e + HALF, x2[i]);
+    }
+  }
+  float rstd = 1.f;
+  if (w) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < CPT; ++i)
+      if (threadIdx.x + i * 256 < n) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += x1[i][e] * x1[i][e] + x2[i][e] * x2[i][e];
+      }
+    rstd = 1.f / sqrtf(block_sum(ss, red) / (float)(heads * HD) + eps);
+  }
+  const float* sn = sin_t + (int64_t)pos * HD;
+  const float* cs = cos_t + (int64_t)pos * HD;
+#pragma unroll
+  for (int i = 0; i < CPT; ++i) {
+    const int c = threadIdx.x + i * 256;
+    if (c >= n) break;  // the lanes of a head leave together
+    const int h = c / CPH, j = (c % CPH) * 8;
+    if (w) {
+      float w1[8], w2[8];
+      ld8f<DT>(w, h * HD + j, w1);
+      ld8f<DT>(w, h * HD + j + HALF, w2);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x1[i][e] = x1[i][e] * rstd * w1[e], x2[i][e] = x2[i][e] * rstd * w2[e];
+    }
+    if (part < 2) {
+      float c1[8], c2[8], s1[8], s2[8];
+      ld8f<O355_F32>(cs, j, c1), ld8f<O355_F32>(cs, j + HALF, c2), ld8f<O355_F32>(sn, j, s1), ld8f<O355_F32>(sn, j + HALF, s2);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float a = x1[i][e], bb = x2[i][e];
+        x1[i][e] = a * c1[e] - bb * s1[e];
+        x2[i][e] = bb * c2[e] + a * s2[e];
+      }
+    }
+    if (part == 0) {
+      st8f<DT>(q_out, row * dq + h * HD + j, x1[i]);
+      st8f<DT>(q_out, row * dq + h * HD + j + HALF, x2[i]);
+      continue;
+    }
+    const int64_t at = ((int64_t)b * Hkv + h) * Lmax + pos;
+    if (kc) {  // the row as the unquantised cache would hold it
+      void* full = part == 1 ? kc : vc;
+      st8f<DT>(full, at * HD + j, x1[i]);
+      st8f<DT>(full, at * HD + j + HALF, x2[i]);
+    }
+    float amax = 0.f;
+    bool finite = true;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float a = fabsf(x1[i][e]), bb = fabsf(x2[i][e]);
+      finite = finite && a <= 3.4028234663852886e38f && bb <= 3.4028234663852886e38f;
+      amax = fmaxf(amax, fmaxf(a, bb));
+    }
+    if (!finite) amax = INFINITY;
+    amax = fmaxf(amax, dpp_lane<0xB1>(amax));                          // quad_perm [1,0,3,2]
+    if constexpr (CPH >= 4) amax = fmaxf(amax, dpp_lane<0x4E>(amax));  // quad_perm [2,3,0,1]
+    if constexpr (CPH >= 8) amax = fmaxf(amax, dpp_lane<0x141>(amax)); // row_half_mirror
+    const bool ok = amax < INFINITY;
+    const float scale = ok ? fmaxf(amax / 127.f, 1.1754943508222875e-38f) : __builtin_nanf("");
+    const float inv = ok ? 1.f / scale : 0.f;
+    auto code = [&](float v) { return ok ? (uint32_t)(uint8_t)(int8_t)(int)rintf(v * inv) : 0u; };
+    u32x2 p1, p2;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      p1[g] = code(x1[i][4 * g]) | code(x1[i][4 * g + 1]) << 8 | code(x1[i][4 * g + 2]) << 16 | code(x1[i][4 * g + 3]) << 24;
+      p2[g] = code(x2[i][4 * g]) | code(x2[i][4 * g + 1]) << 8 | code(x2[i][4 * g + 2]) << 16 | code(x2[i][4 * g + 3]) << 24;
+    }
+    int8_t* codes = part == 1 ? kq : vq;
+    *reinterpret_cast<u32x2*>(codes + at * HD + j) = p1;
+    *reinterpret_cast<u32x2*>(codes + at * HD + j + HALF) = p2;
+    if (j == 0) (part == 1 ? ks : vs)[at] = scale;
+  }
+}
+
+// ---- read back --------------------------------------------------------------------------------------------------
+// A thread turns 16 codes into 16 values; grid.y 0: keys, 1: values.
+template <int DT, int HD>
+__global__ __launch_bounds__(256) void kv_read_q8_kernel(const int8_t* __restrict__ kq, const int8_t* __restrict__ vq,
+                                                         const float* __restrict__ ks, const float* __restrict__ vs,
+                                                         void* __restrict__ kout, void* __restrict__ vout, int64_t pieces, int n,
+                                                         int Lmax, int start, int Lout, int out_start) {
+  constexpr int PPR = HD / 16;  // pieces per row
+  const int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (p >= pieces) return;
+  const int8_t* codes = blockIdx.y ? vq : kq;
+  const float* scales = blockIdx.y ? vs : ks;
+  const int64_t r = p / PPR, bh = r / n, t = r - bh * n;
+  const int c = (int)(p - r * PPR) * 16;
+  const int64_t src = bh * Lmax + start + t, dst = (bh * Lout + out_start + t) * HD + c;
+  const u32x4 w = *reinterpret_cast<const u32x4*>(codes + src * HD + c);
+  const float s = scales[src];
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = (float)(int8_t)(w[2 * g + (e >> 2)] >> (8 * (e & 3))) * s;
+    st8f<DT>(blockIdx.y ? vout : kout, dst + 8 * g, f);
+  }
+}
+
+// ---- decode attention over the codes ------------------------------------------------------------------------------
+// Grid: (sequence, kv head, 16 query heads of the group, run of keys).  See attn_rows.h for what a workgroup does.
+template <int DT, int HD>
+__global__ __launch_bounds__(256, 2) void attn_decode_q8_kernel(const void* __restrict__ q, const int8_t* __restrict__ kq,
+                                                                const int8_t* __restrict__ vq, const float* __restrict__ ks,
+                                                                const float* __restrict__ vs, const float* __restrict__ key_bias,
+                                                                void* __restrict__ out, float* __restrict__ ws, int H, int Hkv,
+                                                                int Lmax, int past_len, const int32_t* __restrict__ past_dev,
+                                                                int n_keys_max, int bias_stride, int tiles, int splits, int64_t rows) {
+  __shared__ RowsLds<HD> lds;
+  const int64_t i = blockIdx.x;
+  const int split = (int)(i % splits);
+  const int64_t i1 = i / splits;
+  const int tile = (int)(i1 % tiles);
+  const int64_t bh = i1 / tiles;
+  const int b = (int)(bh / Hkv), hk = (int)(bh - (int64_t)b * Hkv), G = H / Hkv;
+  const int keys = max(1, min((past_dev ? *past_dev : past_len) + 1, n_keys_max)), steps = (keys + 31) / 32;
+  RowsIn in;
+  in.q = (const unsigned char*)q, in.tok0 = b, in.G = G, in.H = H, in.head0 = hk * G;
+  in.r0 = 16 * tile, in.nrows = min(G, 16 * tile + 16);
+  in.k = (const unsigned char*)kq + bh * Lmax * HD, in.v = (const unsigned char*)vq + bh * Lmax * HD;
+  in.ks = ks + bh * Lmax, in.vs = vs + bh * Lmax;
+  in.bias = key_bias ? key_bias + (int64_t)b * bias_stride : nullptr;
+  in.step_lo = (int)((int64_t)steps * split / splits), in.step_hi = (int)((int64_t)steps * (split + 1) / splits);
+  in.keys = keys, in.past = -1;
+  attend_rows<DT, HD, 1, true, Q8Keys<DT, HD>>(in, lds, [&](int r, int c, auto& o, float m, float l) {
+    constexpr int VC = HD / 16;
+    const int64_t at = (int64_t)b * H + hk * G + r;
+    if (splits == 1) {
+      const float inv = 1.f / l;
+#pragma unroll
+      for (int j = 0; j < VC; ++j) o[j] *= inv;
+      st_row<DT, VC>(out, at * HD + c, o);
+    } else {
+      st_row<O355_F32, VC>(ws, (split * rows + at) * HD + c, o);
+      if (c == 0) {
+        float* ml = ws + rows * splits * HD + (split * rows + at) * 2;
+        ml[0] = m, ml[1] = l;
+      }
+    }
+  });
+}
+
+// Runs of keys per (sequence, kv head, row tile): enough workgroups for two per CU, at least 128 keys each (one step per
+// wave).
+int decode_q8_splits(int B, int H, int Hkv, int n_keys_max) {
+  const int64_t units = (int64_t)B * Hkv * ((H / Hkv + 15) / 16);
+  const int most = (n_keys_max + 127) / 128;
+  const int64_t want = (512 + units - 1) / units;
+  return (int)(want < 1 ? 1 : want > most ? most : want);
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+}  // namespace
+
+#define Q8_SWITCH_HD(hd, DTv, CALL) \
+  switch (hd) {                     \
+    case 32: CALL(DTv, 32); break;  \
+    case 64: CALL(DTv, 64); break;  \
+    case 128: CALL(DTv, 128); break; \
+    default: return O355_EUNSUPPORTED; \
+  }
+#define Q8_SWITCH(dtype, hd, CALL)                             \
+  switch (dtype) {                                             \
+    case O355_F32: Q8_SWITCH_HD(hd, O355_F32, CALL) break;     \
+    case O355_BF16: Q8_SWITCH_HD(hd, O355_BF16, CALL) break;   \
+    case O355_F16: Q8_SWITCH_HD(hd, O355_F16, CALL) break;     \
+    default: return O355_EUNSUPPORTED;                         \
+  }
+
+extern "C" int olmo355_qknorm_rope_kvwrite_q8(const void* qkv, const void* qw, const void* kw, const float* sin_tab,
+                                              const float* cos_tab, void* q_out, int8_t* kq, int8_t* vq, float* kscale,
+                                              float* vscale, void* kcache, void* vcache, int B, int T, int H, int Hkv, int hd,
+                                              int Lmax, int n_pos, int past_len, const int32_t* past_len_dev, float eps, int dtype,
+                                              void* stream) {
+  if (!qkv || !sin_tab || !cos_tab || !q_out || !kq || !vq || !kscale || !vscale) return O355_EINVAL;
+  if (B <= 0 || T <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || Lmax <= 0 || n_pos <= 0 || past_len < 0) return O355_EINVAL;
+  if ((qw == nullptr) != (kw == nullptr) || (kcache == nullptr) != (vcache == nullptr)) return O355_EINVAL;
+  if (!past_len_dev && ((int64_t)past_len + T > Lmax || (int64_t)past_len + T > n_pos)) return O355_EINVAL;
+  for (const void* p : {qkv, qw, kw, (const void*)sin_tab, (const void*)cos_tab, (const void*)q_out, (const void*)kq, (const void*)vq,
+                        (const void*)kcache, (const void*)vcache})
+    if (!aligned16(p)) return O355_EINVAL;
+  if (past_len_dev && T != 1) return O355_EUNSUPPORTED;
+  if (hd != 32 && hd != 64 && hd != 128) return O355_EUNSUPPORTED;
+  const int64_t chunks = (int64_t)H * hd / 16;
+  if (chunks > 1024 || (int64_t)B * T > 0x7fffffff) return O355_EUNSUPPORTED;
+  hipStream_t s = as_stream(stream);
+  const dim3 grid((unsigned)((int64_t)B * T), 3);
+#define WRITE(DTv, HDv, CPT)                                                                                                      \
+  hipLaunchKernelGGL((kv_write_q8_kernel<DTv, HDv, CPT>), grid, dim3(256), 0, s, qkv, qw, kw, sin_tab, cos_tab, q_out, kq, vq,    \
+                     kscale, vscale, kcache, vcache, T, H, Hkv, Lmax, n_pos, past_len, past_len_dev, eps)
+#define WRITE_CPT(DTv, HDv)                  \
+  do {                                       \
+    if (chunks <= 256) WRITE(DTv, HDv, 1);   \
+    else if (chunks <= 512) WRITE(DTv, HDv, 2); \
+    else WRITE(DTv, HDv, 4);                 \
+  } while (0)
+  Q8_SWITCH(dtype, hd, WRITE_CPT)
+#undef WRITE_CPT
+#undef WRITE
+  O355_CHECK_LAUNCH();
+}
+
+extern "C" int olmo355_kv_read_q8(const int8_t* kq, const int8_t* vq, const float* kscale, const float* vscale, void* kout, void* vout,
+                                  int B, int Hkv, int hd, int Lmax, int start, int n, int Lout, int out_start, int dtype, void* stream) {
+  if (!kq || !vq || !kscale || !vscale || !kout || !vout) return O355_EINVAL;
+  if (B <= 0 || Hkv <= 0 || Lmax <= 0 || Lout <= 0 || start < 0 || n <= 0 || out_start < 0) return O355_EINVAL;
+  if ((int64_t)start + n > Lmax || (int64_t)out_start + n > Lout) return O355_EINVAL;
+  for (const void* p : {(const void*)kq, (const void*)vq, (const void*)kout, (const void*)vout})
+    if (!aligned16(p)) return O355_EINVAL;
+  if (hd != 32 && hd != 64 && hd != 128) return O355_EUNSUPPORTED;
+  const int64_t pieces = (int64_t)B * Hkv * n * (hd / 16), blocks = (pieces + 255) / 256;
+  if (blocks > 0x7fffffff) return O355_EUNSUPPORTED;
+  hipStream_t s = as_stream(stream);
+#define READ(DTv, HDv)                                                                                                            \
+  hipLaunchKernelGGL((kv_read_q8_kernel<DTv, HDv>), dim3((unsigned)blocks, 2), dim3(256), 0, s, kq, vq, kscale, vscale, kout, vout, \
+                     pieces, n, Lmax, start, Lout, out_start)
+  Q8_SWITCH(dtype, hd, READ)
+#undef READ
+  O355_CHECK_LAUNCH();
+}
+
+extern "C" int64_t olmo355_attn_decode_q8_workspace_bytes(int B, int H, int Hkv, int hd, int n_keys_max) {
+  if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || hd <= 0 || n_keys_max <= 0) return 0;
+  const int splits = decode_q8_splits(B, H, Hkv, n_keys_max);
+  return splits == 1 ? 0 : 4 * rows_parts_floats((int64_t)B * H, hd, splits);
+}
+
+extern "C" int olmo355_attn_decode_q8(const void* q, const int8_t* kq, const int8_t* vq, const float* kscale, const float* vscale,
+                                      const float* key_bias, void* out, void* ws, int64_t ws_bytes, int B, int H, int Hkv, int hd,
+                                      int Lmax, int past_len, const int32_t* past_len_dev, int n_keys_max, int bias_stride, int dtype,
+                                      void* stream) {
+  if (!q || !kq || !vq || !kscale || !vscale || !out) return O355_EINVAL;
+  if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || past_len < 0 || n_keys_max <= 0 || n_keys_max > Lmax) return O355_EINVAL;
+  if (!past_len_dev && past_len >= n_keys_max) return O355_EINVAL;
+  if (key_bias && bias_stride < n_keys_max) return O355_EINVAL;
+  for (const void* p : {q, (const void*)kq, (const void*)vq, (const void*)out, (const void*)ws})
+    if (!aligned16(p)) return O355_EINVAL;
+  if (hd != 32 && hd != 64 && hd != 128) return O355_EUNSUPPORTED;
+  const int64_t need = olmo355_attn_decode_q8_workspace_bytes(B, H, Hkv, hd, n_keys_max);
+  if (need && (!ws || ws_bytes < need)) return O355_EINVAL;
+  const int tiles = (H / Hkv + 15) / 16, splits = decode_q8_splits(B, H, Hkv, n_keys_max);
+  const int64_t rows = (int64_t)B * H, wgs = (int64_t)B * Hkv * tiles * splits;
+  if (wgs > 0x7fffffff) return O355_EUNSUPPORTED;
+  hipStream_t s = as_stream(stream);
+#define DECODE(DTv, HDv)                                                                                                          \
+  hipLaunchKernelGGL((attn_decode_q8_kernel<DTv, HDv>), dim3((unsigned)wgs), dim3(256), 0, s, q, kq, vq, kscale, vscale, key_bias, \
+                     out, (float*)ws, H, Hkv, Lmax, past_len, past_len_dev, n_keys_max, bias_stride, tiles, splits, rows);         \
+  if (splits > 1)                                                                                                                 \
+  hipLaunchKernelGGL((rows_combine_kernel<DTv, HDv>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, (const float*)ws, out,   \
+                     rows, splits)
+  Q8_SWITCH(dtype, hd, DECODE)
+#undef DECODE
+  O355_CHECK_LAUNCH();
+}

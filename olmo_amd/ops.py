@@ -940,6 +940,190 @@ def attn_decode_fused(qkv, q_weight, k_weight, sin_tab, cos_tab, kcache, vcache,
     return out
 
 
+# ---------------------------------------------------------------------------------------------
+# the cache in 8 bits
+# ---------------------------------------------------------------------------------------------
+@dataclass(frozen=True)
+class KVQ8:
+    """One layer's cache as signed 8-bit codes with one float32 scale per (sequence, kv head, position): about half the
+    bytes of the 16-bit cache.  Written by :func:`qknorm_rope_kvwrite_q8`, attended to by :func:`attn_decode_q8`, read
+    back by :func:`kv_read_q8`."""
+
+    k: torch.Tensor        # int8 [B, Hkv, Lmax, hd], rotated keys
+    v: torch.Tensor
+    k_scale: torch.Tensor  # float32 [B, Hkv, Lmax]
+    v_scale: torch.Tensor
+
+    def __post_init__(self):
+        _dev(self.k, self.v, self.k_scale, self.v_scale)
+        if self.k.dtype != torch.int8 or self.v.dtype != torch.int8 or self.k.dim() != 4 or self.k.shape != self.v.shape:
+            raise TypeError("KVQ8: int8 codes [B, Hkv, Lmax, hd] expected")
+        if any(t.dtype != torch.float32 or t.shape != self.k.shape[:3] for t in (self.k_scale, self.v_scale)):
+            raise TypeError("KVQ8: float32 scales [B, Hkv, Lmax] expected")
+
+    @classmethod
+    def empty(cls, B: int, Hkv: int, Lmax: int, hd: int, device) -> "KVQ8":
+        codes = torch.empty(2, B, Hkv, Lmax, hd, dtype=torch.int8, device=device)
+        scales = torch.empty(2, B, Hkv, Lmax, dtype=torch.float32, device=device)
+        return cls(codes[0], codes[1], scales[0], scales[1])
+
+    def _args(self):
+        return self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr()
+
+
+def _current(t: torch.Tensor) -> None:
+    """Launches go to the current device's stream."""
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"tensors on {t.device}, but the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _past_dev_ok(past_len_dev: Optional[torch.Tensor], T: int) -> None:
+    if past_len_dev is not None and (past_len_dev.dtype != torch.int32 or T != 1):
+        raise ValueError("past_len_dev: a device int32, for one token per sequence")
+
+
+def _key_bias_stride(key_bias: Optional[torch.Tensor], B: int, n: int) -> int:
+    if key_bias is None:
+        return 0
+    if key_bias.dtype != torch.float32 or key_bias.dim() != 2 or key_bias.shape[0] < B or key_bias.shape[1] < n:
+        raise ValueError(f"key_bias: float32 [{B}, at least {n}] expected, got {key_bias.dtype} {tuple(key_bias.shape)}")
+    return key_bias.shape[1]
+
+
+def qknorm_rope_kvwrite_q8(qkv, q_weight, k_weight, sin_tab, cos_tab, cache: KVQ8, B: int, T: int, H: int, Hkv: int, hd: int,
+                           past_len: int, eps: float, past_len_dev: Optional[torch.Tensor] = None,
+                           kcache: Optional[torch.Tensor] = None, vcache: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`qknorm_rope_kvwrite` into an 8-bit cache: returns q (normed + rotated) ``[B, T, H*hd]`` and writes codes and
+    scales of the rotated k and of v.  float32 all the way to the codes (q: to its one rounding).  ``kcache`` /
+    ``vcache`` ``[B, Hkv, Lmax, hd]``, if given, receive the same rows unquantised."""
+    _dev(qkv, q_weight, k_weight, sin_tab, cos_tab, kcache, vcache, past_len_dev, cache.k)
+    _current(qkv)
+    if qkv.shape[-1] != (H + 2 * Hkv) * hd or qkv.numel() != B * T * (H + 2 * Hkv) * hd:
+        raise ValueError("qkv shape mismatch")
+    if cache.k.shape[0] < B or cache.k.shape[1] != Hkv or cache.k.shape[3] != hd:
+        raise ValueError(f"cache shape {tuple(cache.k.shape)} does not fit B={B} Hkv={Hkv} hd={hd}")
+    if (kcache is None) != (vcache is None) or (q_weight is None) != (k_weight is None):
+        raise ValueError("kcache and vcache, q_weight and k_weight: both or neither")
+    Lmax, n_pos = cache.k.shape[2], sin_tab.shape[0]
+    if kcache is not None and (kcache.dtype != qkv.dtype or vcache.dtype != qkv.dtype or kcache.shape != vcache.shape
+                               or kcache.shape != (kcache.shape[0], Hkv, Lmax, hd) or kcache.shape[0] < B):
+        raise ValueError("kcache / vcache: [B, Hkv, Lmax, hd] of qkv's dtype and of the 8-bit cache's length expected")
+    if q_weight is not None and (q_weight.dtype != qkv.dtype or k_weight.dtype != qkv.dtype or q_weight.numel() != H * hd
+                                 or k_weight.numel() != Hkv * hd):
+        raise ValueError("q_weight [H * hd] and k_weight [Hkv * hd] of qkv's dtype expected")
+    if sin_tab.dtype != torch.float32 or cos_tab.dtype != torch.float32 or sin_tab.shape != cos_tab.shape or sin_tab.shape[-1] != hd:
+        raise ValueError("sin/cos tables must be float32 [n_pos, hd]")
+    _past_dev_ok(past_len_dev, T)
+    if past_len_dev is None and not 0 <= past_len <= min(Lmax, n_pos) - T:
+        raise ValueError(f"rows {past_len} .. {past_len + T - 1} outside the cache ({Lmax}) or the rotary table ({n_pos})")
+    q = torch.empty(B, T, H * hd, dtype=qkv.dtype, device=qkv.device)
+    if B * T:
+        check("olmo355_qknorm_rope_kvwrite_q8",
+              lib().olmo355_qknorm_rope_kvwrite_q8(_p(qkv), _p(q_weight), _p(k_weight), _p(sin_tab), _p(cos_tab), _p(q),
+                                                   *cache._args(), _p(kcache), _p(vcache), B, T, H, Hkv, hd, Lmax, n_pos, past_len,
+                                                   _p(past_len_dev), float(eps), _dt(qkv), _stream()))
+    return q
+
+
+def kv_read_q8(cache: KVQ8, start: int, n: int, dtype: torch.dtype,
+               out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows ``start .. start + n - 1`` of an 8-bit cache as values (``code * scale``, one rounding to ``dtype``): new
+    ``(k, v)`` of shape ``[B, Hkv, n, hd]``, or into the same rows of ``out``, a pair of caches ``[B, Hkv, L, hd]``."""
+    B, Hkv, Lmax, hd = cache.k.shape
+    _current(cache.k)
+    if start < 0 or n < 0 or start + n > Lmax:
+        raise ValueError(f"rows {start} .. {start + n - 1} outside the cache of {Lmax}")
+    if out is None:
+        kv = torch.empty(2, B, Hkv, n, hd, dtype=dtype, device=cache.k.device)
+        k, v, at = kv[0], kv[1], 0
+    else:
+        (k, v), at = out, start
+        _dev(k, v, cache.k)
+        if k.dtype != dtype or v.dtype != dtype or k.shape != v.shape or k.dim() != 4 or (k.shape[0], k.shape[1], k.shape[3]) != (B, Hkv, hd):
+            raise ValueError(f"out: two caches [{B}, {Hkv}, L, {hd}] of {dtype} expected")
+        if k.shape[2] < start + n:
+            raise ValueError("out is too short")
+    dt = _dt(k)
+    if n and B:
+        check("olmo355_kv_read_q8",
+              lib().olmo355_kv_read_q8(*cache._args(), _p(k), _p(v), B, Hkv, hd, Lmax, start, n, k.shape[2], at, dt, _stream()))
+    return k, v
+
+
+def attn_decode_q8_workspace(B: int, H: int, Hkv: int, hd: int, n_keys_max: int, device) -> torch.Tensor:
+    n = int(lib().olmo355_attn_decode_q8_workspace_bytes(B, H, Hkv, hd, n_keys_max))
+    return torch.empty(n // 4, dtype=torch.float32, device=device)
+
+
+def attn_decode_q8(q, cache: KVQ8, ws: torch.Tensor, B: int, H: int, Hkv: int, hd: int, past_len: int, n_keys_max: int,
+                   key_bias: Optional[torch.Tensor] = None, past_len_dev: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`attn_decode` over an 8-bit cache: one query per sequence, keys ``0 .. past_len``; ``ws`` from
+    :func:`attn_decode_q8_workspace` (one per stream: overlapping calls must not share it)."""
+    _dev(q, cache.k, ws, key_bias, past_len_dev)
+    _current(q)
+    if q.numel() != B * H * hd:
+        raise ValueError("q shape mismatch")
+    if cache.k.shape[0] < B or cache.k.shape[1] != Hkv or cache.k.shape[3] != hd:
+        raise ValueError(f"cache shape {tuple(cache.k.shape)} does not fit B={B} Hkv={Hkv} hd={hd}")
+    _past_dev_ok(past_len_dev, 1)
+    Lmax = cache.k.shape[2]
+    if not 0 < n_keys_max <= Lmax or (past_len_dev is None and not 0 <= past_len < n_keys_max):
+        raise ValueError(f"past_len {past_len}, n_keys_max {n_keys_max} do not fit a cache of {Lmax}")
+    stride = _key_bias_stride(key_bias, B, n_keys_max)
+    if _nbytes(ws) < int(lib().olmo355_attn_decode_q8_workspace_bytes(B, H, Hkv, hd, n_keys_max)):
+        raise ValueError("attention workspace too small")
+    out = torch.empty(B, 1, H * hd, dtype=q.dtype, device=q.device)
+    check("olmo355_attn_decode_q8",
+          lib().olmo355_attn_decode_q8(_p(q), *cache._args(), _p(key_bias), _p(out), _p(ws), _nbytes(ws), B, H, Hkv, hd, Lmax,
+                                       past_len, _p(past_len_dev), n_keys_max, stride, _dt(q), _stream()))
+    return out
+
+
+# ---------------------------------------------------------------------------------------------
+# a prefix shared by the batch
+# ---------------------------------------------------------------------------------------------
+def attn_shared_prefix_workspace(B: int, T: int, H: int, Hkv: int, hd: int, prefix_len: int, n_keys_max: int, dtype: torch.dtype,
+                                 device) -> torch.Tensor:
+    n = int(lib().olmo355_attn_shared_prefix_workspace_bytes(B, T, H, Hkv, hd, prefix_len, n_keys_max, _DT.get(dtype, -1)))
+    return torch.empty(n // 4, dtype=torch.float32, device=device)
+
+
+def attn_shared_prefix(q, kprefix, vprefix, kcache, vcache, ws: torch.Tensor, B: int, T: int, H: int, Hkv: int, hd: int,
+                       prefix_len: int, past_len: int, n_keys_max: int, key_bias: Optional[torch.Tensor] = None,
+                       past_len_dev: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of ``T`` new tokens per sequence behind a prefix that the whole batch shares: keys ``0 ..
+    prefix_len - 1`` of ``kprefix`` / ``vprefix`` (``[Hkv, P, hd]``, held and read once), then rows ``0 .. past_len + t``
+    of the sequence's own caches ``[B, Hkv, Lmax, hd]`` (already written).  ``key_bias`` ``[B, n]`` is for the own rows; a
+    masked one weighs nothing.  ``ws`` from :func:`attn_shared_prefix_workspace` (one per stream)."""
+    _dev(q, kprefix, vprefix, kcache, vcache, ws, key_bias, past_len_dev)
+    _current(q)
+    if q.numel() != B * T * H * hd:
+        raise ValueError("q shape mismatch")
+    if any(t.dtype != q.dtype for t in (kprefix, vprefix, kcache, vcache)):
+        raise TypeError("prefix and caches must have q's dtype")
+    if kprefix.dim() != 3 or kprefix.shape != vprefix.shape or kprefix.shape[0] != Hkv or kprefix.shape[2] != hd:
+        raise ValueError(f"prefix shape {tuple(kprefix.shape)} is not [Hkv={Hkv}, P, hd={hd}]")
+    if kcache.dim() != 4 or kcache.shape != vcache.shape or kcache.shape[0] < B or kcache.shape[1] != Hkv or kcache.shape[3] != hd:
+        raise ValueError(f"cache shape {tuple(kcache.shape)} does not fit B={B} Hkv={Hkv} hd={hd}")
+    if not 0 < prefix_len <= kprefix.shape[1]:
+        raise ValueError(f"prefix_len {prefix_len} outside 1 .. {kprefix.shape[1]} (without a prefix: attn_prefill / attn_decode)")
+    _past_dev_ok(past_len_dev, T)
+    if n_keys_max > kcache.shape[2] or n_keys_max < T or (past_len_dev is None and not 0 <= past_len <= n_keys_max - T):
+        raise ValueError(f"past_len {past_len} + {T} new tokens, n_keys_max {n_keys_max} do not fit a cache of {kcache.shape[2]}")
+    stride = _key_bias_stride(key_bias, B, n_keys_max)
+    dt = _dt(q)
+    out = torch.empty(B, T, H * hd, dtype=q.dtype, device=q.device)
+    if not out.numel():
+        return out
+    if _nbytes(ws) < int(lib().olmo355_attn_shared_prefix_workspace_bytes(B, T, H, Hkv, hd, prefix_len, n_keys_max, dt)):
+        raise ValueError("attention workspace too small")
+    check("olmo355_attn_shared_prefix",
+          lib().olmo355_attn_shared_prefix(_p(q), _p(kprefix), _p(vprefix), _p(kcache), _p(vcache), _p(key_bias), _p(out), _p(ws),
+                                           _nbytes(ws), B, T, H, Hkv, hd, prefix_len, kprefix.shape[1], kcache.shape[2], past_len,
+                                           _p(past_len_dev), n_keys_max, stride, dt, _stream()))
+    return out
+
+
 def rope_advance(pos_dev: torch.Tensor, delta: int, sin_tab: torch.Tensor, cos_tab: torch.Tensor,
                  rope_now: torch.Tensor) -> None:
     """``pos_dev += delta`` (device int32) and ``rope_now = [sin_tab[pos] | cos_tab[pos]]``: run between
