@@ -19,7 +19,7 @@
 namespace {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef f32x4 f32x4_a4 __attribute__((aligned(4)));
 
 constexpr float kRowsMaskThreshold = -1e30f;  // bias entries at or below: the key is masked
@@ -83,7 +83,7 @@ __device__ __forceinline__ void ld_words(const void* p, uint32_t (&w)[N]) {
 // clamped to the last key): row_k[2] for the two key tiles, row_v[8] for its 8 keys.
 template <int DT, int HD>
 struct RawKeys {
-  static constexpr bool SCALED = false;
+  static constexpr bool SCALED = false, TWO_STAGES = false, REST = false;
   static constexpr int PV = DT;  // type of the second product
   static constexpr int ES = DT == O355_F32 ? 4 : 2, STEPS = HD / 32, VC = HD / 16, VW = VC * ES / 4;
   typename Frag8<DT>::T k[2][STEPS];
@@ -113,18 +113,20 @@ struct RawKeys {
       return __builtin_bit_cast(typename Frag8<DT>::T, w);
     }
   }
-  __device__ __forceinline__ void drop(int e) {  // key e of the lane weighs nothing, whatever its values hold
+  __device__ __forceinline__ void keep(int e, uint32_t ones) {  // ones 0: key e of the lane weighs nothing, whatever its values hold
 #pragma unroll
-    for (int i = 0; i < VW; ++i) v[e][i] = 0;
+    for (int i = 0; i < VW; ++i) v[e][i] &= ones;
   }
 };
 
 // K / V as 8-bit codes.  A 16-byte load holds two steps' worth of a key: its channels 64 i + 16 kq .. + 15.
 template <int DT, int HD>
 struct Q8Keys {
-  static constexpr bool SCALED = true;
-  // The value codes are multiplied with p * scale rounded to bf16 (relative 2^-8 per term, in a sum over keys) for both
-  // 16-bit types: p * scale has no bound that would keep it inside fp16's range.  fp32 activations stay in fp32.
+  static constexpr bool SCALED = true, TWO_STAGES = true;
+  // The value codes are multiplied with p * scale in bf16 for both 16-bit types: p * scale has no bound that would keep it
+  // inside fp16's range.  REST: what the rounding to bf16 left goes through a second product, which keeps 16 bits of every
+  // weight; fp16 results need them.  fp32 activations stay in fp32.
+  static constexpr bool REST = DT != O355_F32;
   static constexpr int PV = DT == O355_F32 ? O355_F32 : O355_BF16;
   static constexpr int STEPS = HD / 32, VC = HD / 16, KW = HD / 16;  // KW: words of a key per lane
   uint32_t k[2][KW];
@@ -166,7 +168,6 @@ struct Q8Keys {
     for (int e = 0; e < 8; ++e) f[e] = code(v[e][j >> 2], j & 3);
     return Frag8<PV>::pack(f);
   }
-  __device__ __forceinline__ void drop(int) {}  // codes are finite; the caller drops the key's scale
 };
 
 // ---- one workgroup: rows x keys -> merged (m, l, o) -----------------------------------------------------------
@@ -183,6 +184,13 @@ struct RowsIn {
   int past;                     // causal: row r sees keys <= past + r / G; -1: all keys
 };
 
+// run `i` of `n` of `steps` steps
+__device__ __forceinline__ void share_steps(RowsIn& in, uint32_t steps, uint32_t i, uint32_t n) {
+  const uint32_t each = steps / n, rest = steps - each * n;
+  in.step_lo = (int)(i * each + min(i, rest));
+  in.step_hi = in.step_lo + (int)(each + (i < rest ? 1 : 0));
+}
+
 template <int HD>
 struct RowsLds {
   static constexpr int PITCH = HD + 4;
@@ -195,6 +203,7 @@ struct RowsLds {
 // emit(row, channel, VC values of o, m, l): called by 16 threads per row, once for every row of the workgroup.
 template <int DT, int HD, int RT, bool KEEP_MASKED, class Keys, class Emit>
 __device__ __forceinline__ void attend_rows(const RowsIn& in, RowsLds<HD>& lds, Emit emit) {
+  const float* const bias = in.bias;
   typedef Frag8<DT> FQ;
   typedef Frag8<Keys::PV> FP;
   constexpr int STEPS = HD / 32, VC = HD / 16, ES = DT == O355_F32 ? 4 : 2;
@@ -210,7 +219,7 @@ __device__ __forceinline__ void attend_rows(const RowsIn& in, RowsLds<HD>& lds, 
   for (int rt = 0; rt < RT; ++rt) {
     const int r = min(in.r0 + 16 * rt + col, in.nrows - 1);
     const int t = r / in.G;
-    sees[rt] = in.past < 0 ? in.keys - 1 : in.past + t;
+    sees[rt] = in.past < 0 ? in.keys - 1 : min(in.past + t, in.keys - 1);
     const unsigned char* src = in.q + (((int64_t)(in.tok0 + t) * in.H + in.head0 + (r - t * in.G)) * HD) * ES;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) qf[rt][s] = FQ::ld(src + Keys::q_elem(s, kq) * ES);
@@ -223,73 +232,81 @@ __device__ __forceinline__ void attend_rows(const RowsIn& in, RowsLds<HD>& lds, 
 #pragma unroll
     for (int j = 0; j < VC; ++j) o[rt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  const bool causal = in.past >= 0;
-
-  for (int step = in.step_lo + wave; step < in.step_hi; step += 4) {
+  // A step's loads.  Per-key numbers (scales, bias): the four lanes of a quad load those of the lane group's four keys of a
+  // tile, one each, and the quad's lanes get them by quad broadcast when they are used.  No load sits in a branch: behind
+  // a join the compiler would have to wait for all loads in flight instead of the older stage's.
+  struct Stage {
+    Keys kv;
+    float sk[2], sv[2], bs[2];
+  };
+  auto request = [&](Stage& g, int step) {
     const int k0 = step * 32, left = in.keys - 1 - k0;  // left >= 0: the last row of the step that exists
-    int row_k[2] = {col, 16 + col}, row_v[8];
+    int row_k[2] = {col, 16 + col}, row_v[8], row_s[2] = {4 * kq + (col & 3), 16 + 4 * kq + (col & 3)};
 #pragma unroll
     for (int e = 0; e < 8; ++e) row_v[e] = 4 * kq + (e & 3) + 16 * (e >> 2);
-    int row_s[2] = {4 * kq, 16 + 4 * kq};  // first of four scale / bias entries
-    const bool tail = left < 31;
-    if (tail) {
+    if (left < 31) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) row_k[i] = min(row_k[i], left);
+      for (int i = 0; i < 2; ++i) row_k[i] = min(row_k[i], left), row_s[i] = min(row_s[i], left);
 #pragma unroll
       for (int e = 0; e < 8; ++e) row_v[e] = min(row_v[e], left);
     }
-    Keys kv;
-    kv.load(in.k + (int64_t)k0 * KROW, in.v + (int64_t)k0 * KROW, row_k, row_v, col, kq);
-    float sk[8], sv[8], bs[8];
-    auto ld8 = [&](const float* p, float (&f)[8]) {
-      if (tail) {
+    g.kv.load(in.k + (int64_t)k0 * KROW, in.v + (int64_t)k0 * KROW, row_k, row_v, col, kq);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = p[row_v[e]];
-      } else {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const f32x4 w = *reinterpret_cast<const f32x4_a4*>(p + row_s[h]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) f[4 * h + e] = w[e];
-        }
-      }
-    };
-    if constexpr (Keys::SCALED) ld8(in.ks + k0, sk), ld8(in.vs + k0, sv);
-    if (in.bias) ld8(in.bias + k0, bs);
-
+    for (int h = 0; h < 2; ++h) {
+      if constexpr (Keys::SCALED) g.sk[h] = in.ks[k0 + row_s[h]], g.sv[h] = in.vs[k0 + row_s[h]];
+      g.bs[h] = bias ? bias[k0 + row_s[h]] : 0.f;
+    }
+  };
+  auto of_quad = [](const float (&f)[2], int e) {  // lane e & 3 of the quad
+    return (e & 3) == 0 ? dpp_lane<0x00>(f[e >> 2]) : (e & 3) == 1 ? dpp_lane<0x55>(f[e >> 2]) : (e & 3) == 2 ? dpp_lane<0xAA>(f[e >> 2]) : dpp_lane<0xFF>(f[e >> 2]);
+  };
+  const int all_see = in.past < 0 ? in.keys - 1 : in.past + in.r0 / in.G;  // the last key that every row sees
+  auto multiply = [&](Stage& g, int step) {
+    const int k0 = step * 32;
     // ---- S^T = K . Q^T
     f32x4 s[RT][2];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int st = 0; st < STEPS; ++st) {
-        const auto kf = kv.kfrag(kt, st);
+        const auto kf = g.kv.kfrag(kt, st);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) s[rt][kt] = FQ::mma(kf, qf[rt][st], st == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[rt][kt]);
       }
-    if (in.bias && !KEEP_MASKED) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (bs[e] <= kRowsMaskThreshold) kv.drop(e);
-    }
-    // ---- running maximum, probabilities
-    typename FP::T pf[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      float x[8], tmax = -INFINITY;
+    if constexpr (Keys::SCALED) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        float v = s[rt][e >> 2][e & 3] * c2;
-        if constexpr (Keys::SCALED) v *= sk[e];
-        if (in.bias) {
-          v = __builtin_fmaf(bs[e], kLog2e, v);
-          v = bs[e] <= kRowsMaskThreshold ? (KEEP_MASKED ? lowest : -INFINITY) : v;
-        }
-        const int key = 4 * kq + (e & 3) + 16 * (e >> 2);
-        if (tail || causal) v = k0 + key > min(sees[rt], in.keys - 1) ? -INFINITY : v;
-        x[e] = v;
-        tmax = fmaxf(tmax, v);
+        const float k = of_quad(g.sk, e);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s[rt][e >> 2][e & 3] *= k;
       }
+    }
+    // scores into the log2 domain: at once where a bias is added or keys are hidden, else inside the exponent
+    const bool hides = k0 + 31 > all_see, plain = !bias && !hides;
+    if (!plain) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float bs = of_quad(g.bs, e), b2 = bs * kLog2e;
+        const bool masked = bs <= kRowsMaskThreshold;
+        if constexpr (!KEEP_MASKED) g.kv.keep(e, masked ? 0u : ~0u);
+        const int key = k0 + 4 * kq + (e & 3) + 16 * (e >> 2);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          float v = __builtin_fmaf(s[rt][e >> 2][e & 3], c2, b2);
+          v = masked ? (KEEP_MASKED ? lowest : -INFINITY) : v;
+          s[rt][e >> 2][e & 3] = key > sees[rt] ? -INFINITY : v;
+        }
+      }
+    }
+    const float cs = plain ? c2 : 1.f;
+    // ---- running maximum, probabilities
+    typename FP::T pf[RT], pl[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float tmax = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) tmax = fmaxf(tmax, s[rt][e >> 2][e & 3]);
+      tmax *= cs;  // cs > 0: the maximum commutes with the scaling
       // The reference maximum moves only when some row's new maximum is more than kRowsLazyMax above it.
       if (__builtin_amdgcn_ballot_w64(tmax > m[rt] + kRowsLazyMax) != 0) {
         tmax = combine_xor32(combine_xor16(tmax, MaxOp{}), MaxOp{});
@@ -306,18 +323,57 @@ __device__ __forceinline__ void attend_rows(const RowsIn& in, RowsLds<HD>& lds, 
       float p[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        p[e] = __builtin_amdgcn_exp2f(x[e] - mref);
+        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][e >> 2][e & 3], cs, -mref));
         l[rt] += p[e];
-        if constexpr (Keys::SCALED) p[e] = p[e] == 0.f ? 0.f : p[e] * sv[e];  // the scale of a key that weighs nothing may be NaN
+        if constexpr (Keys::SCALED) {  // the scale of a key that weighs nothing may be NaN
+          const float v = of_quad(g.sv, e);
+          p[e] = p[e] == 0.f ? 0.f : p[e] * v;
+        }
       }
       pf[rt] = FP::pack(p);
+      if constexpr (Keys::REST) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] -= round_bf16(p[e]);
+        pl[rt] = FP::pack(p);
+      }
     }
     // ---- O^T += V^T . P^T
 #pragma unroll
     for (int j = 0; j < VC; ++j) {
-      const auto vf = kv.vfrag(j);
+      const auto vf = g.kv.vfrag(j);
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) o[rt][j] = FP::mma(vf, pf[rt], o[rt][j]);
+      for (int rt = 0; rt < RT; ++rt) {
+        o[rt][j] = FP::mma(vf, pf[rt], o[rt][j]);
+        if constexpr (Keys::REST) o[rt][j] = FP::mma(vf, pl[rt], o[rt][j]);
+      }
+    }
+  };
+  int step = in.step_lo + wave;
+  if (step < in.step_hi) {
+    Stage a;
+    request(a, step);
+    if constexpr (Keys::TWO_STAGES) {  // the next 32 keys are in flight while the present ones are multiplied
+      Stage b;
+      while (true) {
+        if (step + 4 >= in.step_hi) break;
+        request(b, step + 4);
+        multiply(a, step);
+        step += 4;
+        if (step + 4 >= in.step_hi) {
+          a = b;
+          break;
+        }
+        request(a, step + 4);
+        multiply(b, step);
+        step += 4;
+      }
+      multiply(a, step);
+    } else {
+      while (true) {
+        multiply(a, step);
+        if ((step += 4) >= in.step_hi) break;
+        request(a, step);
+      }
     }
   }
 
@@ -377,33 +433,36 @@ __device__ __forceinline__ void st_row(void* out, int64_t elem, const float (&f)
 // Partial results of rows whose keys several workgroups share: o unnormalised [part][rows][HD], then (m, l) [part][rows].
 __host__ __device__ __forceinline__ int64_t rows_parts_floats(int64_t rows, int hd, int parts) { return rows * parts * (hd + 2); }
 
+// A wave per row: its four groups of 16 lanes take every fourth part, lane c the VC channels c * VC ...
 template <int DT, int HD>
 __global__ __launch_bounds__(256) void rows_combine_kernel(const float* __restrict__ ws, void* __restrict__ out, int64_t rows, int parts) {
   constexpr int VC = HD / 16;
-  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  const int c = (threadIdx.x & 15) * VC;
+  const int lane = threadIdx.x & 63, grp = lane >> 4, c = (lane & 15) * VC;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= rows) return;
-  const float* ml = ws + rows * parts * HD;
-  float mm = -INFINITY, l = 0.f, o[VC];
-  for (int i = 0; i < parts; ++i) mm = fmaxf(mm, ml[(i * rows + row) * 2]);
+  const f32x2* ml = reinterpret_cast<const f32x2*>(ws + rows * parts * HD);
+  float mm = -INFINITY;
+  for (int i = lane; i < parts; i += 64) mm = fmaxf(mm, ml[i * rows + row][0]);
+  mm = wave_max(mm);
+  float l = 0.f, o[VC];
 #pragma unroll
   for (int j = 0; j < VC; ++j) o[j] = 0.f;
-  for (int i = 0; i < parts; ++i) {
-    const float mi = ml[(i * rows + row) * 2], li = ml[(i * rows + row) * 2 + 1];
-    if (mi == -INFINITY) {
-      l += li;  // 0, or NaN from a NaN score
-      continue;
-    }
-    const float w = __builtin_amdgcn_exp2f(mi - mm);
-    l += li * w;
-    if (w == 0.f) continue;
+#pragma unroll 4
+  for (int i = grp; i < parts; i += 4) {
+    const f32x2 p = ml[i * rows + row];
+    const float* src = ws + (i * rows + row) * HD + c;
+    float v[VC];
 #pragma unroll
-    for (int j = 0; j < VC; ++j) o[j] += w * ws[(i * rows + row) * HD + c + j];
+    for (int j = 0; j < VC; ++j) v[j] = src[j];
+    const float w = p[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(p[0] - mm);
+    l += p[0] == -INFINITY ? p[1] : p[1] * w;  // no key seen: 0, or NaN from a NaN score
+#pragma unroll
+    for (int j = 0; j < VC; ++j) o[j] += w == 0.f ? 0.f : w * v[j];
   }
-  const float inv = 1.f / l;
+  l = combine_xor32(combine_xor16(l, AddOp{}), AddOp{});
 #pragma unroll
-  for (int j = 0; j < VC; ++j) o[j] *= inv;
-  st_row<DT, VC>(out, row * HD + c, o);
+  for (int j = 0; j < VC; ++j) o[j] = combine_xor32(combine_xor16(o[j], AddOp{}), AddOp{}) / l;
+  if (grp == 0) st_row<DT, VC>(out, row * HD + c, o);
 }
 
 }  // namespace

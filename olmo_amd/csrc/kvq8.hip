@@ -181,33 +181,30 @@ __global__ __launch_bounds__(256) void kv_read_q8_kernel(const int8_t* __restric
 }
 
 // ---- decode attention over the codes ------------------------------------------------------------------------------
-// Grid: (sequence, kv head, 16 query heads of the group, run of keys).  See attn_rows.h for what a workgroup does.
+// Grid: (16 query heads of the group x run of keys, kv head, sequence).  See attn_rows.h for what a workgroup does.
 template <int DT, int HD>
 __global__ __launch_bounds__(256, 2) void attn_decode_q8_kernel(const void* __restrict__ q, const int8_t* __restrict__ kq,
                                                                 const int8_t* __restrict__ vq, const float* __restrict__ ks,
                                                                 const float* __restrict__ vs, const float* __restrict__ key_bias,
-                                                                void* __restrict__ out, float* __restrict__ ws, int H, int Hkv,
+                                                                void* __restrict__ out, float* __restrict__ ws, int G, int Hkv,
                                                                 int Lmax, int past_len, const int32_t* __restrict__ past_dev,
-                                                                int n_keys_max, int bias_stride, int tiles, int splits, int64_t rows) {
+                                                                int n_keys_max, int bias_stride, int splits, int64_t rows) {
   __shared__ RowsLds<HD> lds;
-  const int64_t i = blockIdx.x;
-  const int split = (int)(i % splits);
-  const int64_t i1 = i / splits;
-  const int tile = (int)(i1 % tiles);
-  const int64_t bh = i1 / tiles;
-  const int b = (int)(bh / Hkv), hk = (int)(bh - (int64_t)b * Hkv), G = H / Hkv;
-  const int keys = max(1, min((past_dev ? *past_dev : past_len) + 1, n_keys_max)), steps = (keys + 31) / 32;
+  const uint32_t tile = blockIdx.x / (uint32_t)splits, split = blockIdx.x - tile * splits;
+  const int hk = blockIdx.y, b = blockIdx.z;
+  const int64_t bh = (int64_t)b * Hkv + hk;
+  const int keys = max(1, min((past_dev ? *past_dev : past_len) + 1, n_keys_max));
   RowsIn in;
-  in.q = (const unsigned char*)q, in.tok0 = b, in.G = G, in.H = H, in.head0 = hk * G;
-  in.r0 = 16 * tile, in.nrows = min(G, 16 * tile + 16);
+  in.q = (const unsigned char*)q, in.tok0 = b, in.G = G, in.H = Hkv * G, in.head0 = hk * G;
+  in.r0 = 16 * tile, in.nrows = min(G, in.r0 + 16);
   in.k = (const unsigned char*)kq + bh * Lmax * HD, in.v = (const unsigned char*)vq + bh * Lmax * HD;
   in.ks = ks + bh * Lmax, in.vs = vs + bh * Lmax;
   in.bias = key_bias ? key_bias + (int64_t)b * bias_stride : nullptr;
-  in.step_lo = (int)((int64_t)steps * split / splits), in.step_hi = (int)((int64_t)steps * (split + 1) / splits);
   in.keys = keys, in.past = -1;
+  share_steps(in, (uint32_t)(keys + 31) / 32, split, splits);
   attend_rows<DT, HD, 1, true, Q8Keys<DT, HD>>(in, lds, [&](int r, int c, auto& o, float m, float l) {
     constexpr int VC = HD / 16;
-    const int64_t at = (int64_t)b * H + hk * G + r;
+    const int64_t at = bh * G + r;
     if (splits == 1) {
       const float inv = 1.f / l;
 #pragma unroll
@@ -323,14 +320,15 @@ extern "C" int olmo355_attn_decode_q8(const void* q, const int8_t* kq, const int
   const int64_t need = olmo355_attn_decode_q8_workspace_bytes(B, H, Hkv, hd, n_keys_max);
   if (need && (!ws || ws_bytes < need)) return O355_EINVAL;
   const int tiles = (H / Hkv + 15) / 16, splits = decode_q8_splits(B, H, Hkv, n_keys_max);
-  const int64_t rows = (int64_t)B * H, wgs = (int64_t)B * Hkv * tiles * splits;
-  if (wgs > 0x7fffffff) return O355_EUNSUPPORTED;
+  const int64_t rows = (int64_t)B * H;
+  if (B > 65535 || Hkv > 65535) return O355_EUNSUPPORTED;  // grid limits
+  const dim3 grid(tiles * splits, Hkv, B);
   hipStream_t s = as_stream(stream);
 #define DECODE(DTv, HDv)                                                                                                          \
-  hipLaunchKernelGGL((attn_decode_q8_kernel<DTv, HDv>), dim3((unsigned)wgs), dim3(256), 0, s, q, kq, vq, kscale, vscale, key_bias, \
-                     out, (float*)ws, H, Hkv, Lmax, past_len, past_len_dev, n_keys_max, bias_stride, tiles, splits, rows);         \
+  hipLaunchKernelGGL((attn_decode_q8_kernel<DTv, HDv>), grid, dim3(256), 0, s, q, kq, vq, kscale, vscale, key_bias, out,             \
+                     (float*)ws, H / Hkv, Hkv, Lmax, past_len, past_len_dev, n_keys_max, bias_stride, splits, rows);               \
   if (splits > 1)                                                                                                                 \
-  hipLaunchKernelGGL((rows_combine_kernel<DTv, HDv>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, (const float*)ws, out,   \
+  hipLaunchKernelGGL((rows_combine_kernel<DTv, HDv>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, (const float*)ws, out,   \
                      rows, splits)
   Q8_SWITCH(dtype, hd, DECODE)
 #undef DECODE

@@ -13,7 +13,7 @@ struct PrefixPlan {
   int rtp, rto;          // 16-row tiles per workgroup, prefix part and own part
   int tiles_p, tiles_o;  // row tiles per kv head (prefix) and per sequence and kv head (own)
   int splits_p, splits_o;
-  int64_t wgs_p, wgs_o;
+  int64_t wgs_p, wgs_o;    // workgroups per kv head
 };
 
 PrefixPlan prefix_plan(int B, int T, int H, int Hkv, int P, int n_keys_max, int dtype) {
@@ -30,19 +30,19 @@ PrefixPlan prefix_plan(int B, int T, int H, int Hkv, int P, int n_keys_max, int 
   };
   p.splits_p = splits((int64_t)Hkv * p.tiles_p, P, 512);
   p.splits_o = splits((int64_t)B * Hkv * p.tiles_o, n_keys_max, 512);
-  p.wgs_p = (int64_t)Hkv * p.tiles_p * p.splits_p;
-  p.wgs_o = (int64_t)B * Hkv * p.tiles_o * p.splits_o;
+  p.wgs_p = (int64_t)p.tiles_p * p.splits_p;
+  p.wgs_o = (int64_t)B * p.tiles_o * p.splits_o;
   return p;
 }
 
 template <int DT, int HD, int RTP, int RTO>
-__global__ __launch_bounds__(256, 1) void attn_shared_prefix_kernel(
+__global__ __launch_bounds__(256, (RTP <= 2 && (DT != O355_F32 || HD < 128) ? 2 : 1)) void attn_shared_prefix_kernel(
     const void* __restrict__ q, const void* __restrict__ kp, const void* __restrict__ vp, const void* __restrict__ kc,
-    const void* __restrict__ vc, const float* __restrict__ key_bias, float* __restrict__ ws, int B, int T, int H, int Hkv, int P,
+    const void* __restrict__ vc, const float* __restrict__ key_bias, float* __restrict__ ws, int B, int T, int G, int Hkv, int P,
     int64_t Pmax, int64_t Lmax, int past_len, const int32_t* __restrict__ past_dev, int n_keys_max, int bias_stride, PrefixPlan plan) {
   constexpr int ES = DT == O355_F32 ? 4 : 2, VC = HD / 16;
   __shared__ RowsLds<HD> lds;
-  const int G = H / Hkv;
+  const int H = Hkv * G;
   const int64_t rows = (int64_t)B * T * H;
   const int parts = plan.splits_p + plan.splits_o;
   RowsIn in;
@@ -57,25 +57,23 @@ __global__ __launch_bounds__(256, 1) void attn_shared_prefix_kernel(
       ml[0] = m, ml[1] = l;
     }
   };
-  int64_t i = blockIdx.x;
-  if (i < plan.wgs_p) {
-    part = (int)(i % plan.splits_p);
-    i /= plan.splits_p;
-    const int tile = (int)(i % plan.tiles_p), hk = (int)(i / plan.tiles_p), steps = (P + 31) / 32;
+  const int hk = blockIdx.y;
+  uint32_t i = blockIdx.x;
+  if (i < (uint32_t)plan.wgs_p) {
+    const uint32_t tile = i / (uint32_t)plan.splits_p;
+    part = (int)(i - tile * plan.splits_p);
     in.tok0 = 0, in.head0 = hk * G;
     in.r0 = tile * 16 * RTP, in.nrows = B * T * G;
     in.k = (const unsigned char*)kp + hk * Pmax * HD * ES, in.v = (const unsigned char*)vp + hk * Pmax * HD * ES;
     in.bias = nullptr, in.keys = P, in.past = -1;
-    in.step_lo = (int)((int64_t)steps * part / plan.splits_p), in.step_hi = (int)((int64_t)steps * (part + 1) / plan.splits_p);
+    share_steps(in, (uint32_t)(P + 31) / 32, part, plan.splits_p);
     attend_rows<DT, HD, RTP, false, RawKeys<DT, HD>>(in, lds, emit);
     return;
   }
-  i -= plan.wgs_p;
-  const int split = (int)(i % plan.splits_o);
-  i /= plan.splits_o;
-  const int tile = (int)(i % plan.tiles_o);
-  const int64_t bh = i / plan.tiles_o;
-  const int b = (int)(bh / Hkv), hk = (int)(bh - (int64_t)b * Hkv);
+  i -= (uint32_t)plan.wgs_p;
+  const uint32_t i1 = i / (uint32_t)plan.splits_o, split = i - i1 * plan.splits_o;
+  const uint32_t b = i1 / (uint32_t)plan.tiles_o, tile = i1 - b * plan.tiles_o;
+  const int64_t bh = (int64_t)b * Hkv + hk;
   const int past = past_dev ? max(0, min(*past_dev, n_keys_max - 1)) : past_len;
   part = plan.splits_p + split;
   in.tok0 = b * T, in.head0 = hk * G;
@@ -84,8 +82,7 @@ __global__ __launch_bounds__(256, 1) void attn_shared_prefix_kernel(
   in.k = (const unsigned char*)kc + bh * Lmax * HD * ES, in.v = (const unsigned char*)vc + bh * Lmax * HD * ES;
   in.bias = key_bias ? key_bias + (int64_t)b * bias_stride : nullptr;
   in.keys = last + 1, in.past = past;
-  const int steps = (last + 32) / 32;
-  in.step_lo = (int)((int64_t)steps * split / plan.splits_o), in.step_hi = (int)((int64_t)steps * (split + 1) / plan.splits_o);
+  share_steps(in, (uint32_t)(last + 32) / 32, split, plan.splits_o);
   attend_rows<DT, HD, RTO, false, RawKeys<DT, HD>>(in, lds, emit);
 }
 
@@ -96,10 +93,11 @@ int launch_shared_prefix(const void* q, const void* kp, const void* vp, const vo
                          float* ws, int B, int T, int H, int Hkv, int P, int64_t Pmax, int64_t Lmax, int past_len,
                          const int32_t* past_dev, int n_keys_max, int bias_stride, const PrefixPlan& plan, hipStream_t s) {
   const int64_t wgs = plan.wgs_p + plan.wgs_o, rows = (int64_t)B * T * H;
-  if (wgs > 0x7fffffff || (rows + 15) / 16 > 0x7fffffff) return O355_EUNSUPPORTED;
+  if (wgs > 0x7fffffff || (rows + 3) / 4 > 0x7fffffff || Hkv > 65535) return O355_EUNSUPPORTED;  // grid limits
+  const dim3 grid((unsigned)wgs, Hkv);
 #define RUN(RTP, RTO)                                                                                                              \
-  hipLaunchKernelGGL((attn_shared_prefix_kernel<DT, HD, RTP, RTO>), dim3((unsigned)wgs), dim3(256), 0, s, q, kp, vp, kc, vc, key_bias, \
-                     ws, B, T, H, Hkv, P, Pmax, Lmax, past_len, past_dev, n_keys_max, bias_stride, plan)
+  hipLaunchKernelGGL((attn_shared_prefix_kernel<DT, HD, RTP, RTO>), grid, dim3(256), 0, s, q, kp, vp, kc, vc, key_bias, \
+                     ws, B, T, H / Hkv, Hkv, P, Pmax, Lmax, past_len, past_dev, n_keys_max, bias_stride, plan)
   if (plan.rtp == 1) RUN(1, 1);
   else if (plan.rtp == 2 && plan.rto == 1) RUN(2, 1);
   else if (plan.rtp == 2) RUN(2, 2);
@@ -108,7 +106,7 @@ int launch_shared_prefix(const void* q, const void* kp, const void* vp, const vo
     else RUN(4, 4);
   }
 #undef RUN
-  hipLaunchKernelGGL((rows_combine_kernel<DT, HD>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, (const float*)ws, out, rows,
+  hipLaunchKernelGGL((rows_combine_kernel<DT, HD>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, (const float*)ws, out, rows,
                      plan.splits_p + plan.splits_o);
   O355_CHECK_LAUNCH();
 }
