@@ -14,6 +14,8 @@
 //   The 8 keys of lane group kq are 4 kq .. + 3 and 16 + 4 kq .. + 3 of the 32: where the accumulators of S^T already
 //   sit, so the probabilities go from accumulators to the second product inside the lane.
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
@@ -83,18 +85,19 @@ __device__ __forceinline__ void ld_words(const void* p, uint32_t (&w)[N]) {
 // clamped to the last key): row_k[2] for the two key tiles, row_v[8] for its 8 keys.
 template <int DT, int HD>
 struct RawKeys {
-  static constexpr bool SCALED = false, TWO_STAGES = false, REST = false;
+  static constexpr bool SCALED = false, REST = false;
   static constexpr int PV = DT;  // type of the second product
   static constexpr int ES = DT == O355_F32 ? 4 : 2, STEPS = HD / 32, VC = HD / 16, VW = VC * ES / 4;
   typename Frag8<DT>::T k[2][STEPS];
   uint32_t v[8][VW];
   static __device__ __forceinline__ int q_elem(int s, int kq) { return 32 * s + 8 * kq; }
-  __device__ __forceinline__ void load(const unsigned char* kb, const unsigned char* vb, const int (&row_k)[2], const int (&row_v)[8],
-                                       int col, int kq) {
+  __device__ __forceinline__ void load_k(const unsigned char* kb, const int (&row_k)[2], int kq) {
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) k[kt][s] = Frag8<DT>::ld(kb + (uint32_t)(row_k[kt] * (HD * ES) + (32 * s + 8 * kq) * ES));
+  }
+  __device__ __forceinline__ void load_v(const unsigned char* vb, const int (&row_v)[8], int col) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) ld_words<VW>(vb + (uint32_t)(row_v[e] * (HD * ES) + col * (VC * ES)), v[e]);
   }
@@ -122,7 +125,7 @@ struct RawKeys {
 // K / V as 8-bit codes.  A 16-byte load holds two steps' worth of a key: its channels 64 i + 16 kq .. + 15.
 template <int DT, int HD>
 struct Q8Keys {
-  static constexpr bool SCALED = true, TWO_STAGES = true;
+  static constexpr bool SCALED = true;
   // The value codes are multiplied with p * scale in bf16 for both 16-bit types: p * scale has no bound that would keep it
   // inside fp16's range.  REST: what the rounding to bf16 left goes through a second product, which keeps 16 bits of every
   // weight; fp16 results need them.  fp32 activations stay in fp32.
@@ -132,8 +135,7 @@ struct Q8Keys {
   uint32_t k[2][KW];
   u32x2 v[8];  // VC codes: 8, 4 or 2 of the bytes
   static __device__ __forceinline__ int q_elem(int s, int kq) { return HD == 32 ? 8 * kq : 64 * (s >> 1) + 16 * kq + 8 * (s & 1); }
-  __device__ __forceinline__ void load(const unsigned char* kb, const unsigned char* vb, const int (&row_k)[2], const int (&row_v)[8],
-                                       int col, int kq) {
+  __device__ __forceinline__ void load_k(const unsigned char* kb, const int (&row_k)[2], int kq) {
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
       if constexpr (HD == 32) {
@@ -147,6 +149,8 @@ struct Q8Keys {
         }
       }
     }
+  }
+  __device__ __forceinline__ void load_v(const unsigned char* vb, const int (&row_v)[8], int col) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const unsigned char* p = vb + (uint32_t)(row_v[e] * HD + col * VC);
@@ -170,7 +174,7 @@ struct Q8Keys {
   }
 };
 
-// ---- one workgroup: rows x keys -> merged (m, l, o) -----------------------------------------------------------
+// ---- rows x keys -> (m, l, o) -----------------------------------------------------------
 struct RowsIn {
   const unsigned char* q;  // the activation rows [token][H][HD]
   int tok0;                // row r belongs to token tok0 + r / G, head head0 + r % G
@@ -179,16 +183,17 @@ struct RowsIn {
   const unsigned char *k, *v;   // this kv head's keys and values, row 0
   const float *ks, *vs;         // scales of the 8-bit form
   const float* bias;            // per key, or NULL
-  int step_lo, step_hi;         // runs of 32 keys
   int keys;                     // keys in all (rows past them are not read)
   int past;                     // causal: row r sees keys <= past + r / G; -1: all keys
 };
 
 // run `i` of `n` of `steps` steps
-__device__ __forceinline__ void share_steps(RowsIn& in, uint32_t steps, uint32_t i, uint32_t n) {
-  const uint32_t each = steps / n, rest = steps - each * n;
-  in.step_lo = (int)(i * each + min(i, rest));
-  in.step_hi = in.step_lo + (int)(each + (i < rest ? 1 : 0));
+struct Run {
+  int lo, hi;
+};
+__device__ __forceinline__ Run run_of(uint32_t steps, uint32_t i, uint32_t n) {
+  const uint32_t each = steps / n, rest = steps - each * n, lo = i * each + min(i, rest);
+  return {(int)lo, (int)(lo + each + (i < rest ? 1 : 0))};
 }
 
 template <int HD>
@@ -198,20 +203,28 @@ struct RowsLds {
   float o[4][16][PITCH];
 };
 
+template <int HD, int RT>
+struct RowsAcc {  // O^T: lane (row = l & 15, kq) holds channels (4 kq + r) * VC + j of its row in o[.][j][r]
+  f32x4 o[RT][HD / 16];
+  float m[RT], l[RT];  // l: this lane's share (its 8 of every 32 keys)
+};
+
+// One wave: its rows over the runs of 32 keys step_lo, step_lo + stride, ... < step_hi.
 // What a row's masked keys count: KEEP_MASKED: a masked key keeps the type's lowest value as its score (so a row of nothing
 // but masked keys averages them, as the decode attention does); otherwise it weighs nothing.
-// emit(row, channel, VC values of o, m, l): called by 16 threads per row, once for every row of the workgroup.
-template <int DT, int HD, int RT, bool KEEP_MASKED, class Keys, class Emit>
-__device__ __forceinline__ void attend_rows(const RowsIn& in, RowsLds<HD>& lds, Emit emit) {
-  const float* const bias = in.bias;
+template <int DT, int HD, int RT, bool KEEP_MASKED, class Keys>
+__device__ __forceinline__ void walk_keys(const RowsIn& in, int step_lo, int step_hi, int stride, RowsAcc<HD, RT>& acc) {
   typedef Frag8<DT> FQ;
   typedef Frag8<Keys::PV> FP;
   constexpr int STEPS = HD / 32, VC = HD / 16, ES = DT == O355_F32 ? 4 : 2;
   constexpr int KROW = Keys::SCALED ? HD : HD * ES;  // bytes of a key row
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int col = lane & 15, kq = lane >> 4;
+  const float* const bias = in.bias;
+  const int lane = threadIdx.x & 63, col = lane & 15, kq = lane >> 4;
   const float c2 = kLog2e / sqrtf((float)HD);  // scores in the log2 domain
   const float lowest = Act<DT>::lowest();
+  auto& o = acc.o;
+  auto& m = acc.m;
+  auto& l = acc.l;
 
   typename FQ::T qf[RT][STEPS];
   int sees[RT];  // last key visible to the row
@@ -223,60 +236,68 @@ __device__ __forceinline__ void attend_rows(const RowsIn& in, RowsLds<HD>& lds, 
     const unsigned char* src = in.q + (((int64_t)(in.tok0 + t) * in.H + in.head0 + (r - t * in.G)) * HD) * ES;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) qf[rt][s] = FQ::ld(src + Keys::q_elem(s, kq) * ES);
-  }
-  f32x4 o[RT][VC];
-  float m[RT], l[RT];  // l: this lane's share (8 of 32 keys)
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
     m[rt] = -INFINITY, l[rt] = 0.f;
 #pragma unroll
     for (int j = 0; j < VC; ++j) o[rt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  // A step's loads.  Per-key numbers (scales, bias): the four lanes of a quad load those of the lane group's four keys of a
-  // tile, one each, and the quad's lanes get them by quad broadcast when they are used.  No load sits in a branch: behind
-  // a join the compiler would have to wait for all loads in flight instead of the older stage's.
-  struct Stage {
-    Keys kv;
-    float sk[2], sv[2], bs[2];
-  };
-  auto request = [&](Stage& g, int step) {
+  if (step_lo >= step_hi) return;
+  const int all_see = in.past < 0 ? in.keys - 1 : in.past + in.r0 / in.G;  // the last key that every row sees
+
+  // The loads of the next 32 keys go out as soon as the registers of the present ones are free: K after the first product, V
+  // after the second, so that one of them is on its way at any time without a second set of registers.  No load sits in a
+  // branch: behind a join the compiler would have to wait for all loads in flight instead of the older half.
+  // Per-key numbers (scales, bias): the four lanes of a quad load those of the lane group's four keys of a tile, one each,
+  // and get the others' by quad broadcast when they are used.
+  Keys kv;
+  float sk[2], sv[2], bs[2], next_sk[2], next_sv[2], next_bs[2];
+  auto request_k = [&](int step) {
     const int k0 = step * 32, left = in.keys - 1 - k0;  // left >= 0: the last row of the step that exists
-    int row_k[2] = {col, 16 + col}, row_v[8], row_s[2] = {4 * kq + (col & 3), 16 + 4 * kq + (col & 3)};
+    int row_k[2] = {col, 16 + col}, row_s[2] = {4 * kq + (col & 3), 16 + 4 * kq + (col & 3)};
+    if (left < 31) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) row_k[i] = min(row_k[i], left), row_s[i] = min(row_s[i], left);
+    }
+    kv.load_k(in.k + (int64_t)k0 * KROW, row_k, kq);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if constexpr (Keys::SCALED) next_sk[h] = in.ks[k0 + row_s[h]], next_sv[h] = in.vs[k0 + row_s[h]];
+      next_bs[h] = bias ? bias[k0 + row_s[h]] : 0.f;
+    }
+  };
+  auto request_v = [&](int step) {
+    const int k0 = step * 32, left = in.keys - 1 - k0;
+    int row_v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) row_v[e] = 4 * kq + (e & 3) + 16 * (e >> 2);
     if (left < 31) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) row_k[i] = min(row_k[i], left), row_s[i] = min(row_s[i], left);
-#pragma unroll
       for (int e = 0; e < 8; ++e) row_v[e] = min(row_v[e], left);
     }
-    g.kv.load(in.k + (int64_t)k0 * KROW, in.v + (int64_t)k0 * KROW, row_k, row_v, col, kq);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if constexpr (Keys::SCALED) g.sk[h] = in.ks[k0 + row_s[h]], g.sv[h] = in.vs[k0 + row_s[h]];
-      g.bs[h] = bias ? bias[k0 + row_s[h]] : 0.f;
-    }
+    kv.load_v(in.v + (int64_t)k0 * KROW, row_v, col);
   };
   auto of_quad = [](const float (&f)[2], int e) {  // lane e & 3 of the quad
     return (e & 3) == 0 ? dpp_lane<0x00>(f[e >> 2]) : (e & 3) == 1 ? dpp_lane<0x55>(f[e >> 2]) : (e & 3) == 2 ? dpp_lane<0xAA>(f[e >> 2]) : dpp_lane<0xFF>(f[e >> 2]);
   };
-  const int all_see = in.past < 0 ? in.keys - 1 : in.past + in.r0 / in.G;  // the last key that every row sees
-  auto multiply = [&](Stage& g, int step) {
+  auto multiply = [&](int step, auto more) {
+    constexpr bool MORE = decltype(more)::value;
     const int k0 = step * 32;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) sk[h] = next_sk[h], sv[h] = next_sv[h], bs[h] = next_bs[h];
     // ---- S^T = K . Q^T
     f32x4 s[RT][2];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int st = 0; st < STEPS; ++st) {
-        const auto kf = g.kv.kfrag(kt, st);
+        const auto kf = kv.kfrag(kt, st);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) s[rt][kt] = FQ::mma(kf, qf[rt][st], st == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[rt][kt]);
       }
+    if constexpr (MORE) request_k(step + stride);
     if constexpr (Keys::SCALED) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float k = of_quad(g.sk, e);
+        const float k = of_quad(sk, e);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) s[rt][e >> 2][e & 3] *= k;
       }
@@ -286,9 +307,9 @@ __device__ __forceinline__ void attend_rows(const RowsIn& in, RowsLds<HD>& lds, 
     if (!plain) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float bs = of_quad(g.bs, e), b2 = bs * kLog2e;
-        const bool masked = bs <= kRowsMaskThreshold;
-        if constexpr (!KEEP_MASKED) g.kv.keep(e, masked ? 0u : ~0u);
+        const float b1 = of_quad(bs, e), b2 = b1 * kLog2e;
+        const bool masked = b1 <= kRowsMaskThreshold;
+        if constexpr (!KEEP_MASKED) kv.keep(e, masked ? 0u : ~0u);
         const int key = k0 + 4 * kq + (e & 3) + 16 * (e >> 2);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -316,7 +337,7 @@ __device__ __forceinline__ void attend_rows(const RowsIn& in, RowsLds<HD>& lds, 
 #pragma unroll
         for (int j = 0; j < VC; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) o[rt][j][r] = alpha == 0.f ? 0.f : o[rt][j][r] * alpha;  // see `weigh`
+          for (int r = 0; r < 4; ++r) o[rt][j][r] = alpha == 0.f ? 0.f : o[rt][j][r] * alpha;  // see merge_waves
         m[rt] = mn;
       }
       const float mref = m[rt] == -INFINITY ? 0.f : m[rt];  // a row that has seen no key yet
@@ -326,7 +347,7 @@ __device__ __forceinline__ void attend_rows(const RowsIn& in, RowsLds<HD>& lds, 
         p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][e >> 2][e & 3], cs, -mref));
         l[rt] += p[e];
         if constexpr (Keys::SCALED) {  // the scale of a key that weighs nothing may be NaN
-          const float v = of_quad(g.sv, e);
+          const float v = of_quad(sv, e);
           p[e] = p[e] == 0.f ? 0.f : p[e] * v;
         }
       }
@@ -340,44 +361,32 @@ __device__ __forceinline__ void attend_rows(const RowsIn& in, RowsLds<HD>& lds, 
     // ---- O^T += V^T . P^T
 #pragma unroll
     for (int j = 0; j < VC; ++j) {
-      const auto vf = g.kv.vfrag(j);
+      const auto vf = kv.vfrag(j);
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         o[rt][j] = FP::mma(vf, pf[rt], o[rt][j]);
         if constexpr (Keys::REST) o[rt][j] = FP::mma(vf, pl[rt], o[rt][j]);
       }
     }
+    if constexpr (MORE) request_v(step + stride);
   };
-  int step = in.step_lo + wave;
-  if (step < in.step_hi) {
-    Stage a;
-    request(a, step);
-    if constexpr (Keys::TWO_STAGES) {  // the next 32 keys are in flight while the present ones are multiplied
-      Stage b;
-      while (true) {
-        if (step + 4 >= in.step_hi) break;
-        request(b, step + 4);
-        multiply(a, step);
-        step += 4;
-        if (step + 4 >= in.step_hi) {
-          a = b;
-          break;
-        }
-        request(a, step + 4);
-        multiply(b, step);
-        step += 4;
-      }
-      multiply(a, step);
-    } else {
-      while (true) {
-        multiply(a, step);
-        if ((step += 4) >= in.step_hi) break;
-        request(a, step);
-      }
-    }
-  }
+  request_k(step_lo);
+  request_v(step_lo);
+  int step = step_lo;
+  for (; step + stride < step_hi; step += stride) multiply(step, std::true_type{});
+  multiply(step, std::false_type{});
+}
 
-  // ---- the four waves' results into one
+// The results of a workgroup's four waves, which took every fourth run of 32 keys, as one.
+// emit(row, channel, VC values of o, m, l): called by 16 threads per row, once for every row of the workgroup.
+template <int HD, int RT, class Emit>
+__device__ __forceinline__ void merge_waves(const RowsIn& in, RowsAcc<HD, RT>& acc, RowsLds<HD>& lds, Emit emit) {
+  constexpr int VC = HD / 16;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, kq = lane >> 4;
+  auto& o = acc.o;
+  auto& m = acc.m;
+  auto& l = acc.l;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     l[rt] = combine_xor32(combine_xor16(l[rt], AddOp{}), AddOp{});
@@ -389,8 +398,8 @@ __device__ __forceinline__ void attend_rows(const RowsIn& in, RowsLds<HD>& lds, 
     float mm = -INFINITY;
 #pragma unroll
     for (int w = 0; w < 4; ++w) mm = fmaxf(mm, lds.m[w][16 * rt + col]);
-    // weigh: what a wave gathered under a maximum that turns out to weigh nothing is left out, not multiplied by zero: it
-    // may be the mean of masked keys' values, which are not looked at once the row has a key that is not masked
+    // What a wave gathered under a maximum that turns out to weigh nothing is left out, not multiplied by zero: it may be the
+    // mean of masked keys' values, which are not looked at once the row has a key that is not masked.
     const float alpha = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rt] - mm);
     if (in.r0 + 16 * rt + col < in.nrows) {
 #pragma unroll

@@ -201,8 +201,10 @@ __global__ __launch_bounds__(256, 2) void attn_decode_q8_kernel(const void* __re
   in.ks = ks + bh * Lmax, in.vs = vs + bh * Lmax;
   in.bias = key_bias ? key_bias + (int64_t)b * bias_stride : nullptr;
   in.keys = keys, in.past = -1;
-  share_steps(in, (uint32_t)(keys + 31) / 32, split, splits);
-  attend_rows<DT, HD, 1, true, Q8Keys<DT, HD>>(in, lds, [&](int r, int c, auto& o, float m, float l) {
+  const Run run = run_of((uint32_t)(keys + 31) / 32, split, splits);
+  RowsAcc<HD, 1> acc;
+  walk_keys<DT, HD, 1, true, Q8Keys<DT, HD>>(in, run.lo + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), run.hi, 4, acc);
+  merge_waves<HD, 1>(in, acc, lds, [&](int r, int c, auto& o, float m, float l) {
     constexpr int VC = HD / 16;
     const int64_t at = bh * G + r;
     if (splits == 1) {
