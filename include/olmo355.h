@@ -308,12 +308,12 @@ int olmo355_rope_advance(int32_t* pos, int delta, const float* sin_tab, const fl
  * (olmo/model.py:615-620). */
 /* olmo355_qknorm_rope_kvwrite into that form: q_out [B*T, H*hd] in the activation type, codes and scales of rows
  * past_len + t.  fp32 from qkv to q's one rounding and to the codes (no rounding between norm, rotation and
- * quantisation).  kcache / vcache: both NULL, or [B, Hkv, Lmax, hd] in the activation type, which receive the same
+ * quantisation).  kcache / vcache: both NULL, or [B, Hkv, Lfull, hd] in the activation type, which receive the same
  * rows unquantised (for a prefill's own attention).  past_len_dev needs T == 1; a position outside the cache or the tables
  * then writes nothing.  H*hd up to 16384. */
 int olmo355_qknorm_rope_kvwrite_q8(const void* qkv, const void* qw, const void* kw, const float* sin_tab,
                                    const float* cos_tab, void* q_out, int8_t* kq, int8_t* vq, float* kscale, float* vscale,
-                                   void* kcache, void* vcache, int B, int T, int H, int Hkv, int hd, int Lmax, int n_pos,
+                                   void* kcache, void* vcache, int Lfull, int B, int T, int H, int Hkv, int hd, int Lmax, int n_pos,
                                    int past_len, const int32_t* past_len_dev, float eps, int dtype, void* stream);
 /* Rows start .. start + n - 1 of every (sequence, kv head) back as values: code * scale, one rounding to `dtype`, into
  * rows out_start .. of kout / vout [B, Hkv, Lout, hd]. */

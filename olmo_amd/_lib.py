@@ -61,7 +61,7 @@ EXPORTS = {
     "olmo355_attn_decode_static": (I, [P, P, P, P, P, I, I, I, I, I, I, P, I, I, I, P]),
     "olmo355_attn_decode_fused": (I, [P, P, P, P, P, P, P, P, P, P, L, I, I, I, I, I, I, I, P, I, I, F, P, P, I, P]),
     "olmo355_attn_decode_beam": (I, [P, P, P, P, P, P, L, I, I, I, I, I, I, P, I, I, P, I, I, I, I, P]),
-    "olmo355_qknorm_rope_kvwrite_q8": (I, [P] * 12 + [I] * 8 + [P, F, I, P]),
+    "olmo355_qknorm_rope_kvwrite_q8": (I, [P] * 12 + [I] * 9 + [P, F, I, P]),
     "olmo355_kv_read_q8": (I, [P] * 6 + [I] * 9 + [P]),
     "olmo355_attn_decode_q8_workspace_bytes": (L, [I, I, I, I, I]),
     "olmo355_attn_decode_q8": (I, [P] * 8 + [L] + [I] * 6 + [P, I, I, I, P]),

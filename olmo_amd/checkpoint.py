@@ -146,7 +146,7 @@ def _iter_tensors(path: str) -> Iterator[Tuple[str, torch.Tensor]]:
 def from_quantized(model_name_or_path: str, device="cuda:0", use_safetensors: Optional[bool] = None,
                    quantize_config: Optional[BaseQuantizeConfig] = None, model_basename: Optional[str] = None,
                    dtype: torch.dtype = torch.bfloat16, max_cache_len: Optional[int] = None,
-                   free_checkpoint_buffers: bool = False):
+                   free_checkpoint_buffers: bool = False, kv_cache: Optional[str] = None):
     """``from_quantized`` (``_base.py:784-918``) for a local directory: read the configs, build the HF-style
     model with ``QuantLinear`` in place of the block Linears, load every tensor by name straight to the GPU,
     build the kernel layouts.  Returns ``(hf_model, quantize_config)``."""
@@ -171,7 +171,7 @@ def from_quantized(model_name_or_path: str, device="cuda:0", use_safetensors: Op
 
     mc = ModelConfig.from_dict(cj)
     hf_cfg = OLMoConfig.from_model_config(mc, use_cache=bool(cj.get("use_cache", False)))
-    model = OLMo(mc, device=device, dtype=dtype, max_cache_len=max_cache_len, block_weight_device="meta")
+    model = OLMo(mc, device=device, dtype=dtype, max_cache_len=max_cache_len, block_weight_device="meta", kv_cache=kv_cache)
     hf = OLMoForCausalLM(hf_cfg, model=model)
     layers = [n for n in _linear_names(hf) if n.startswith(OLMoGPTQForCausalLM.layers_block_name + ".")]
     from .qlinear import make_quant
@@ -238,7 +238,7 @@ def make_state_dict_compatible(state_dict: Dict[str, torch.Tensor], config: Mode
 
 
 def load_unsharded_checkpoint(checkpoint_dir: str, device="cuda:0", dtype: torch.dtype = torch.bfloat16,
-                              max_cache_len: Optional[int] = None):
+                              max_cache_len: Optional[int] = None, kv_cache: Optional[str] = None):
     """``OLMo.from_checkpoint`` for the unsharded layout (``olmo/model.py:1730-1764``): ``config.yaml``
     (its ``model`` section) plus ``model.pt`` (or ``model.safetensors``).  Sharded checkpoints belong to the
     training side and are not read here."""
@@ -254,7 +254,7 @@ def load_unsharded_checkpoint(checkpoint_dir: str, device="cuda:0", dtype: torch
     if path is None:
         raise FileNotFoundError(f"{checkpoint_dir}: no model.pt / model.safetensors (sharded checkpoints are not supported)")
     sd = make_state_dict_compatible(dict(_iter_tensors(path)), mc)
-    model = OLMo(mc, device=device, dtype=dtype, max_cache_len=max_cache_len)
+    model = OLMo(mc, device=device, dtype=dtype, max_cache_len=max_cache_len, kv_cache=kv_cache)
     model.load_reference_state_dict(sd)
     return model.post_init().eval()
 

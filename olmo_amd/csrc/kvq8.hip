@@ -55,7 +55,7 @@ __global__ __launch_bounds__(256) void kv_write_q8_kernel(const void* __restrict
                                                           const void* __restrict__ kw, const float* __restrict__ sin_t,
                                                           const float* __restrict__ cos_t, void* __restrict__ q_out,
                                                           int8_t* __restrict__ kq, int8_t* __restrict__ vq, float* __restrict__ ks,
-                                                          float* __restrict__ vs, void* __restrict__ kc, void* __restrict__ vc, int T,
+                                                          float* __restrict__ vs, void* __restrict__ kc, void* __restrict__ vc, int Lfull, int T,
                                                           int H, int Hkv, int Lmax, int n_pos, int past_len,
                                                           const int32_t* __restrict__ past_dev, float eps) {
   constexpr int CPH = HD / 16, HALF = HD / 2;
@@ -120,10 +120,11 @@ __global__ __launch_bounds__(256) void kv_write_q8_kernel(const void* __restrict
       continue;
     }
     const int64_t at = ((int64_t)b * Hkv + h) * Lmax + pos;
-    if (kc) {  // the row as the unquantised cache would hold it
+    if (kc && pos < Lfull) {  // the row as the unquantised cache would hold it
       void* full = part == 1 ? kc : vc;
-      st8f<DT>(full, at * HD + j, x1[i]);
-      st8f<DT>(full, at * HD + j + HALF, x2[i]);
+      const int64_t e = (((int64_t)b * Hkv + h) * Lfull + pos) * HD + j;
+      st8f<DT>(full, e, x1[i]);
+      st8f<DT>(full, e + HALF, x2[i]);
     }
     float amax = 0.f;
     bool finite = true;
@@ -252,12 +253,13 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 extern "C" int olmo355_qknorm_rope_kvwrite_q8(const void* qkv, const void* qw, const void* kw, const float* sin_tab,
                                               const float* cos_tab, void* q_out, int8_t* kq, int8_t* vq, float* kscale,
-                                              float* vscale, void* kcache, void* vcache, int B, int T, int H, int Hkv, int hd,
+                                              float* vscale, void* kcache, void* vcache, int Lfull, int B, int T, int H, int Hkv, int hd,
                                               int Lmax, int n_pos, int past_len, const int32_t* past_len_dev, float eps, int dtype,
                                               void* stream) {
   if (!qkv || !sin_tab || !cos_tab || !q_out || !kq || !vq || !kscale || !vscale) return O355_EINVAL;
   if (B <= 0 || T <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || Lmax <= 0 || n_pos <= 0 || past_len < 0) return O355_EINVAL;
   if ((qw == nullptr) != (kw == nullptr) || (kcache == nullptr) != (vcache == nullptr)) return O355_EINVAL;
+  if (kcache && (Lfull <= 0 || (!past_len_dev && (int64_t)past_len + T > Lfull))) return O355_EINVAL;
   if (!past_len_dev && ((int64_t)past_len + T > Lmax || (int64_t)past_len + T > n_pos)) return O355_EINVAL;
   for (const void* p : {qkv, qw, kw, (const void*)sin_tab, (const void*)cos_tab, (const void*)q_out, (const void*)kq, (const void*)vq,
                         (const void*)kcache, (const void*)vcache})
@@ -270,7 +272,7 @@ extern "C" int olmo355_qknorm_rope_kvwrite_q8(const void* qkv, const void* qw, c
   const dim3 grid((unsigned)((int64_t)B * T), 3);
 #define WRITE(DTv, HDv, CPT)                                                                                                      \
   hipLaunchKernelGGL((kv_write_q8_kernel<DTv, HDv, CPT>), grid, dim3(256), 0, s, qkv, qw, kw, sin_tab, cos_tab, q_out, kq, vq,    \
-                     kscale, vscale, kcache, vcache, T, H, Hkv, Lmax, n_pos, past_len, past_len_dev, eps)
+                     kscale, vscale, kcache, vcache, Lfull, T, H, Hkv, Lmax, n_pos, past_len, past_len_dev, eps)
 #define WRITE_CPT(DTv, HDv)                  \
   do {                                       \
     if (chunks <= 256) WRITE(DTv, HDv, 1);   \

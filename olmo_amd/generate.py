@@ -91,11 +91,11 @@ class DecodeSession:
 
 
 def _prefill(model, input_ids, attention_mask, sampling: Optional[dict] = None,
-             attention_bias: Optional[torch.Tensor] = None, key_bias_extra: Optional[torch.Tensor] = None):
+             attention_bias: Optional[torch.Tensor] = None, key_bias_extra: Optional[torch.Tensor] = None, prefix=None):
     """``key_bias_extra``: ``attention_bias`` as a per-key bias over prompt + new tokens (see
     ``OLMo.key_bias_from_attention_bias``), for the decode steps that follow."""
     out = model(input_ids, attention_mask=attention_mask, attention_bias=attention_bias, use_cache=True,
-                last_logits_only=True)
+                last_logits_only=True, prefix=prefix)
     cache = out.attn_key_values[0].cache
     B = input_ids.shape[0]
     if sampling is None:
@@ -118,24 +118,26 @@ def _prefill(model, input_ids, attention_mask, sampling: Optional[dict] = None,
 def greedy_generate(model, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor], max_new_tokens: int,
                     use_graph: bool = True, eos_token_id: Optional[int] = None, pad_token_id: Optional[int] = None,
                     return_scores: bool = False, return_logits: bool = False, sampling: Optional[dict] = None,
-                    stop_when_all_ended: bool = False, attention_bias: Optional[torch.Tensor] = None):
+                    stop_when_all_ended: bool = False, attention_bias: Optional[torch.Tensor] = None, prefix=None):
     """Returns ``tokens [B, max_new_tokens]`` (and, on request, the summed log-probabilities of the
     chosen tokens and / or the per-step logits).  Runs ``max_new_tokens`` steps; with
     ``eos_token_id`` the tokens after a sequence's first EOS are replaced by ``pad_token_id`` and add nothing to
     the score, and with ``stop_when_all_ended`` the loop also ends (and the result is cut) once every sequence has
     emitted it, as the reference's search does.
     ``sampling`` (``temperature``, ``top_k``, ``top_p``, ``seed``) draws the tokens instead of taking the
-    arg-max; the same seed and prompt give the same tokens."""
+    arg-max; the same seed and prompt give the same tokens.  ``prefix`` (``OLMo.share_prefix``): ``input_ids`` and
+    ``attention_mask`` are what follows a prompt that the whole batch shares."""
     if max_new_tokens < 1:
         raise ValueError("max_new_tokens must be >= 1")
     input_ids = input_ids.to(model.device)
     B, T0 = input_ids.shape
-    if T0 + max_new_tokens - 1 > model.max_cache_len:
-        raise ValueError(f"prompt {T0} + {max_new_tokens} new tokens exceeds max_cache_len {model.max_cache_len}")
+    shared = prefix.length if prefix is not None else 0
+    if shared + T0 + max_new_tokens - 1 > model.max_cache_len:
+        raise ValueError(f"prompt {shared + T0} + {max_new_tokens} new tokens exceeds max_cache_len {model.max_cache_len}")
     key_bias_extra = None
     if attention_bias is not None:  # olmo/model.py:1607,1645-1651: one bias over prompt + generated tokens
         key_bias_extra = model.key_bias_from_attention_bias(attention_bias, B, 0, T0 + max_new_tokens - 1)
-    out, cache, first, key_bias_full = _prefill(model, input_ids, attention_mask, sampling, attention_bias, key_bias_extra)
+    out, cache, first, key_bias_full = _prefill(model, input_ids, attention_mask, sampling, attention_bias, key_bias_extra, prefix)
     sess = DecodeSession(model, cache, first, key_bias_full, sampling)
     tokens = torch.empty(B, max_new_tokens, dtype=torch.int64, device=model.device)
     tokens[:, 0] = sess.ids.view(B)

@@ -154,7 +154,7 @@ if HAVE_TRANSFORMERS:
             if L == 0:
                 return
             idx = beam_idx.to(self.kv.k[0].device)
-            for t in (*self.kv.k, *self.kv.v):
+            for t in self.kv.row_tensors():
                 t[:, :, :L] = t[:, :, :L].index_select(0, idx)
 
         def crop(self, tokens_to_remove: int) -> None:
@@ -166,11 +166,9 @@ if HAVE_TRANSFORMERS:
 
         def _rebatch(self, pick) -> None:
             old, L = self.kv, self.kv.length
-            k0 = pick(old.k[0][:, :, :L])
-            new = KVCache(len(old.k), k0.shape[0], k0.shape[1], old.capacity, k0.shape[3], k0.dtype, k0.device)
-            for i in range(len(old.k)):
-                new.k[i][:, :, :L] = pick(old.k[i][:, :, :L])
-                new.v[i][:, :, :L] = pick(old.v[i][:, :, :L])
+            new = old.like(pick(old.k[0][:, :, :L]).shape[0])
+            for dst, src in zip(new.row_tensors(), old.row_tensors()):
+                dst[:, :, :L] = pick(src[:, :, :L])
             new.set_length(L)
             self.kv = new
             self.refresh()

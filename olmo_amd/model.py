@@ -15,6 +15,10 @@ KV cache.  The reference returns per layer ``(k, v)`` of shape ``[B, n_kv_heads,
 views ``[:, :, :L]`` into it.  Passing them back as ``past_key_values`` continues in place with
 no copy.  Plain tensors passed as ``past_key_values`` are taken to be in the reference's
 form and are rotated into a fresh cache first.
+
+``OLMo(kv_cache="int8")`` keeps the cache as 8-bit codes with a scale per row (:class:`QuantKVCache`), about half
+the bytes of a 16-bit one.  ``OLMo.share_prefix`` computes a prompt's keys and values once for batches of
+sequences that all begin with it (``prefix=`` of ``forward`` and ``generate``).
 """
 
 from __future__ import annotations
@@ -29,7 +33,7 @@ from . import ops
 from .config import ModelConfig, OLMoConfigurationError
 from .qlinear import QuantLinear
 
-__all__ = ["OLMo", "OLMoOutput", "OLMoGenerateOutput", "LayerKV", "KVCache", "DenseLinear"]
+__all__ = ["OLMo", "OLMoOutput", "OLMoGenerateOutput", "LayerKV", "KVCache", "QuantKVCache", "SharedPrefix", "DenseLinear"]
 
 
 class OLMoOutput(NamedTuple):
@@ -57,6 +61,9 @@ class KVCache:
         kv = torch.empty(2, n_layers, B, Hkv, capacity, hd, dtype=dtype, device=device)
         self.k = list(kv[0].unbind(0))
         self.v = list(kv[1].unbind(0))
+        self._books(B, capacity, device)
+
+    def _books(self, B: int, capacity: int, device) -> None:
         self.B, self.capacity, self.length = B, capacity, 0
         # device copy of the number of cached positions, for captured decode steps
         self.length_dev = torch.zeros(1, dtype=torch.int32, device=device)
@@ -70,6 +77,63 @@ class KVCache:
     def set_length(self, L: int) -> None:
         self.length = L
         self.length_dev.fill_(L)
+
+    def layer(self, i: int):
+        """What layer ``i``'s attention reads and writes."""
+        return self.k[i], self.v[i]
+
+    def row_tensors(self) -> List[torch.Tensor]:
+        """Every tensor ``[B, Hkv, capacity, ...]`` that the cached rows consist of."""
+        return [*self.k, *self.v]
+
+    def like(self, B: int) -> "KVCache":
+        """An empty cache of another batch size."""
+        k = self.k[0]
+        return KVCache(len(self.k), B, k.shape[1], self.capacity, k.shape[3], k.dtype, k.device)
+
+
+class QuantKVCache(KVCache):
+    """The cache in 8 bits: per layer int8 codes ``[B, n_kv_heads, capacity, hd]`` (keys rotated) and a float32
+    scale per row.  ``k`` / ``v`` are the codes: the views handed out as ``attn_key_values`` are to be passed back, not
+    computed with (``ops.kv_read_q8`` reads rows back as values)."""
+
+    def __init__(self, n_layers: int, B: int, Hkv: int, capacity: int, hd: int, device):
+        codes = torch.empty(2, n_layers, B, Hkv, capacity, hd, dtype=torch.int8, device=device)
+        scales = torch.empty(2, n_layers, B, Hkv, capacity, dtype=torch.float32, device=device)
+        self.layers = [ops.KVQ8(codes[0, i], codes[1, i], scales[0, i], scales[1, i]) for i in range(n_layers)]
+        self.k = [q.k for q in self.layers]
+        self.v = [q.v for q in self.layers]
+        self._books(B, capacity, device)
+
+    def layer(self, i: int):
+        return self.layers[i], None
+
+    def row_tensors(self) -> List[torch.Tensor]:
+        return [t for q in self.layers for t in (q.k, q.v, q.k_scale, q.v_scale)]
+
+    def like(self, B: int) -> "QuantKVCache":
+        k = self.k[0]
+        return QuantKVCache(len(self.k), B, k.shape[1], self.capacity, k.shape[3], k.device)
+
+
+class SharedPrefix:
+    """Keys and values of a prompt that many sequences begin with (:meth:`OLMo.share_prefix`): per layer
+    ``[n_kv_heads, length, hd]``, held once however many sequences use it."""
+
+    def __init__(self, k: List[torch.Tensor], v: List[torch.Tensor], length: int):
+        self.k, self.v, self.length = k, v, length
+
+
+class PrefixedKVCache(KVCache):
+    """The sequences' own rows behind a :class:`SharedPrefix`: row ``i`` is position ``prefix.length + i``."""
+
+    def __init__(self, prefix: SharedPrefix, n_layers: int, B: int, Hkv: int, capacity: int, hd: int, dtype, device):
+        super().__init__(n_layers, B, Hkv, capacity, hd, dtype, device)
+        self.prefix = prefix
+
+    def like(self, B: int) -> "PrefixedKVCache":
+        k = self.k[0]
+        return PrefixedKVCache(self.prefix, len(self.k), B, k.shape[1], self.capacity, k.shape[3], k.dtype, k.device)
 
 
 class BeamKVCache(KVCache):
@@ -261,11 +325,17 @@ class _RelayState:
 
 class OLMo(nn.Module):
     def __init__(self, config: ModelConfig, device="cuda", dtype: torch.dtype = torch.bfloat16,
-                 max_cache_len: Optional[int] = None, block_weight_device=None):
+                 max_cache_len: Optional[int] = None, block_weight_device=None, kv_cache: Optional[str] = None):
         """``block_weight_device='meta'`` leaves the four dense Linears of every block unallocated
-        (for models whose block Linears are about to be replaced by ``QuantLinear``)."""
+        (for models whose block Linears are about to be replaced by ``QuantLinear``).  ``kv_cache``: ``None`` (the
+        activation dtype) or ``"int8"``: 8-bit codes with a scale per cached row.  With ``"int8"`` a prompt attends to its own
+        keys and values unrounded and to earlier ones as they are stored; beam search and shared prefixes keep their
+        caches in the activation dtype and are refused."""
         super().__init__()
         config.validate_for_inference()
+        if kv_cache not in (None, "int8"):
+            raise OLMoConfigurationError(f"kv_cache must be None or 'int8', not {kv_cache!r}")
+        self.kv_cache = kv_cache
         if dtype not in (torch.bfloat16, torch.float16, torch.float32):
             raise OLMoConfigurationError("activation dtype must be bfloat16, float16 or float32")
         self.config = config
@@ -285,7 +355,7 @@ class OLMo(nn.Module):
         self._prepared = False
         self._act_order = False
         self._rope: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
-        self._attn_ws: Dict[Tuple[int, int], torch.Tensor] = {}
+        self._attn_ws: Dict[tuple, torch.Tensor] = {}
         self._scratch_kv: Dict[Tuple[int, int], Tuple[torch.Tensor, torch.Tensor]] = {}
 
     # ------------------------------------------------------------------------------------------
@@ -334,6 +404,7 @@ class OLMo(nn.Module):
         self._relay: Optional[_RelayState] = None  # state of the one-row decode relay, made on first use
         self._rope_now = None  # rotary rows of the current position during a captured decode step
         self._beam = None  # the beam cache while a beam-search step runs
+        self._shared: Optional[SharedPrefix] = None  # the prefix while tokens behind one run
         self._prepared = True
         return self
 
@@ -367,6 +438,8 @@ class OLMo(nn.Module):
     # ------------------------------------------------------------------------------------------
     def new_cache(self, B: int, capacity: Optional[int] = None) -> KVCache:
         c = self.config
+        if self.kv_cache == "int8":
+            return QuantKVCache(c.n_layers, B, c.effective_n_kv_heads, capacity or self.max_cache_len, c.head_dim, self.device)
         return KVCache(c.n_layers, B, c.effective_n_kv_heads, capacity or self.max_cache_len, c.head_dim, self.dtype,
                        self.device)
 
@@ -381,10 +454,36 @@ class OLMo(nn.Module):
             kt = k.to(self.device, self.dtype).transpose(1, 2).reshape(B * L, Hkv * hd)
             vt = v.to(self.device, self.dtype).transpose(1, 2).reshape(B * L, Hkv * hd)
             qkv = torch.cat((kt, kt, vt), dim=-1).contiguous()
-            ops.qknorm_rope_kvwrite(qkv, None, None, sin, cos, cache.k[i], cache.v[i], B, L, Hkv, Hkv, hd, 0,
-                                    c.layer_norm_eps)
+            if isinstance(cache, QuantKVCache):
+                ops.qknorm_rope_kvwrite_q8(qkv, None, None, sin, cos, cache.layers[i], B, L, Hkv, Hkv, hd, 0, c.layer_norm_eps)
+            else:
+                ops.qknorm_rope_kvwrite(qkv, None, None, sin, cos, cache.k[i], cache.v[i], B, L, Hkv, Hkv, hd, 0,
+                                        c.layer_norm_eps)
         cache.set_length(L)
         return cache
+
+    @torch.no_grad()
+    def share_prefix(self, prefix_ids: torch.Tensor) -> SharedPrefix:
+        """Run a prompt once and keep its keys and values for any number of sequences that begin with it: pass the
+        result as ``prefix=`` to :meth:`forward` or :meth:`generate`, whose ``input_ids`` are then what follows the
+        prefix.  ``prefix_ids``: ``[P]`` or ``[1, P]``, at least one token."""
+        if self.kv_cache is not None:
+            raise NotImplementedError("a shared prefix is kept in the activation dtype: not with kv_cache='int8'")
+        ids = prefix_ids.view(1, -1)
+        P = ids.shape[1]
+        if P < 1 or P >= self.max_cache_len:
+            raise ValueError(f"a prefix of {P} tokens leaves no room in max_cache_len {self.max_cache_len}")
+        cache = self(ids, use_cache=True, last_logits_only=True).attn_key_values[0].cache
+        ops.streamk_check()
+        return SharedPrefix([k[0, :, :P].contiguous() for k in cache.k], [v[0, :, :P].contiguous() for v in cache.v], P)
+
+    def _prefixed_cache(self, prefix: SharedPrefix, B: int) -> PrefixedKVCache:
+        c = self.config
+        if len(prefix.k) != c.n_layers or prefix.k[0].dtype != self.dtype or tuple(prefix.k[0].shape) != (
+                c.effective_n_kv_heads, prefix.length, c.head_dim):
+            raise ValueError("the prefix was computed by another model")
+        return PrefixedKVCache(prefix, c.n_layers, B, c.effective_n_kv_heads, self.max_cache_len - prefix.length, c.head_dim,
+                               self.dtype, self.device)
 
     def _scratch_cache(self, B: int, T: int):
         key = (B, T)
@@ -405,6 +504,23 @@ class OLMo(nn.Module):
             self._attn_ws[key] = ops.attn_decode_workspace(B, c.n_heads, c.head_dim, key[1], self.device)
         return self._attn_ws[key]
 
+    def _q8_ws(self, B: int, n_keys_max: int) -> torch.Tensor:
+        """The same for the decode attention over an 8-bit cache."""
+        key = ("q8", B, -(-n_keys_max // 1024) * 1024)
+        if key not in self._attn_ws:
+            c = self.config
+            self._attn_ws[key] = ops.attn_decode_q8_workspace(B, c.n_heads, c.effective_n_kv_heads, c.head_dim, key[2], self.device)
+        return self._attn_ws[key]
+
+    def _prefix_ws(self, B: int, P: int, n_keys_max: int) -> torch.Tensor:
+        """Workspace of a decode step behind a shared prefix, kept: captured steps go on using it."""
+        key = ("prefix", B, P, n_keys_max)
+        if key not in self._attn_ws:
+            c = self.config
+            self._attn_ws[key] = ops.attn_shared_prefix_workspace(B, 1, c.n_heads, c.effective_n_kv_heads, c.head_dim, P, n_keys_max,
+                                                                  self.dtype, self.device)
+        return self._attn_ws[key]
+
     # ------------------------------------------------------------------------------------------
     # one block: olmo/model.py:728-823 (wiring), :588-654 (attention)
     # ------------------------------------------------------------------------------------------
@@ -417,6 +533,10 @@ class OLMo(nn.Module):
         sin, cos = self._rope
         qw = blk.q_norm.weight.data if blk.q_norm is not None else None
         kw = blk.k_norm.weight.data if blk.k_norm is not None else None
+        if isinstance(kc, ops.KVQ8):
+            return self._attention_q8(qkv, qw, kw, kc, B, T, past_len, key_bias, graph_pos, n_keys_max)
+        if self._shared is not None:
+            return self._attention_shared(blk.layer_id, qkv, qw, kw, kc, vc, B, T, past_len, key_bias, graph_pos, n_keys_max)
         decode = T == 1 and (graph_pos is not None or past_len > 0)
         beam = self._beam
         if decode and beam is None:
@@ -436,6 +556,40 @@ class OLMo(nn.Module):
             return ops.attn_decode(q, kc, vc, self._decode_ws(B, n_keys_max), B, H, Hkv, hd, past_len, n_keys_max,
                                    key_bias=key_bias, past_len_dev=graph_pos)
         return ops.attn_prefill(q, kc, vc, B, T, H, Hkv, hd, past_len, key_bias=key_bias)
+
+    def _attention_q8(self, qkv, qw, kw, layer: ops.KVQ8, B, T, past_len, key_bias, graph_pos, n_keys_max):
+        """Attention over an 8-bit cache: one token per sequence reads the codes; several are attended to in the
+        activation dtype (earlier rows read back, the new ones as they are) while their codes are stored."""
+        c = self.config
+        H, Hkv, hd = c.n_heads, c.effective_n_kv_heads, c.head_dim
+        sin, cos = self._rope
+        if T == 1:
+            q = ops.qknorm_rope_kvwrite_q8(qkv, qw, kw, sin, cos, layer, B, T, H, Hkv, hd, past_len, c.layer_norm_eps,
+                                           past_len_dev=graph_pos)
+            return ops.attn_decode_q8(q, layer, self._q8_ws(B, n_keys_max), B, H, Hkv, hd, past_len, n_keys_max, key_bias=key_bias,
+                                      past_len_dev=graph_pos)
+        kc, vc = self._scratch_cache(B, past_len + T)
+        if past_len:
+            ops.kv_read_q8(layer, 0, past_len, self.dtype, out=(kc, vc))
+        q = ops.qknorm_rope_kvwrite_q8(qkv, qw, kw, sin, cos, layer, B, T, H, Hkv, hd, past_len, c.layer_norm_eps, kcache=kc, vcache=vc)
+        return ops.attn_prefill(q, kc, vc, B, T, H, Hkv, hd, past_len, key_bias=key_bias)
+
+    def _attention_shared(self, layer_id, qkv, qw, kw, kc, vc, B, T, past_len, key_bias, graph_pos, n_keys_max):
+        """Attention behind a shared prefix: the own rows' positions follow the prefix's."""
+        c, prefix = self.config, self._shared
+        H, Hkv, hd, P = c.n_heads, c.effective_n_kv_heads, c.head_dim, prefix.length
+        sin, cos = self._rope
+        q = ops.qknorm_rope_kvwrite(qkv, qw, kw, sin[P:], cos[P:], kc, vc, B, T, H, Hkv, hd, past_len, c.layer_norm_eps,
+                                    past_len_dev=graph_pos)
+        if T == 1:  # one workspace and one split of the keys for every step, eager or captured
+            n_keys_max = kc.shape[2]
+            ws = self._prefix_ws(B, P, n_keys_max)
+        else:
+            ws = ops.attn_shared_prefix_workspace(B, T, H, Hkv, hd, P, n_keys_max, self.dtype, self.device)
+        if key_bias is not None and key_bias.shape[1] < n_keys_max:
+            key_bias = torch.nn.functional.pad(key_bias, (0, n_keys_max - key_bias.shape[1]))  # not visible: any value
+        return ops.attn_shared_prefix(q, prefix.k[layer_id], prefix.v[layer_id], kc, vc, ws, B, T, H, Hkv, hd, P, past_len, n_keys_max,
+                                      key_bias=key_bias, past_len_dev=graph_pos)
 
     def _block(self, blk: OLMoSequentialBlock, x, kc, vc, B, T, past_len, key_bias, graph_pos, n_keys_max):
         c = self.config
@@ -655,7 +809,11 @@ class OLMo(nn.Module):
         output_hidden_states: Optional[bool] = None,
         doc_lens: Optional[torch.Tensor] = None,
         max_doc_lens: Optional[Sequence[int]] = None,
+        prefix: Optional[SharedPrefix] = None,
     ) -> OLMoOutput:
+        """``olmo/model.py:1253-1465``.  ``prefix`` (of :meth:`share_prefix`): every sequence continues that prompt;
+        ``input_ids``, ``attention_mask`` and the returned cache then hold what follows it (a cache that was begun with a
+        prefix remembers it)."""
         c = self.config
         if doc_lens is not None or max_doc_lens is not None:
             raise NotImplementedError("intra-document masking is a training feature and is not implemented")
@@ -684,13 +842,21 @@ class OLMo(nn.Module):
                 past_len = cache.length
             if cache.B != B:
                 raise ValueError("batch size differs from the cache's")
+            if prefix is not None and getattr(cache, "prefix", None) is not prefix:
+                raise ValueError("the cache was not begun with this prefix")
             if past_len + T > cache.capacity:
                 raise ValueError(f"KV cache capacity {cache.capacity} exceeded ({past_len}+{T}); "
                                  "construct the model with a larger max_cache_len")
         else:
             past_len = 0
-            if use_cache:
+            if prefix is not None:
+                cache = self._prefixed_cache(prefix, B)
+                if T > cache.capacity:
+                    raise ValueError(f"prefix {prefix.length} + {T} tokens exceed max_cache_len {self.max_cache_len}")
+            elif use_cache:
                 cache = self.new_cache(B, max(self.max_cache_len, T))
+        if attention_bias is not None and isinstance(cache, PrefixedKVCache):
+            raise NotImplementedError("attention_bias behind a shared prefix")
 
         # ---- padding mask -> additive per-key bias (olmo/model.py:1337-1340) ---------------------
         key_bias = None
@@ -747,13 +913,14 @@ class OLMo(nn.Module):
         self._rope_now = cache.rope_now if (cache is not None and graph_pos is not None) else None
         hidden: List[torch.Tensor] = []
         self._beam = cache if isinstance(cache, BeamKVCache) else None
+        self._shared = cache.prefix if isinstance(cache, PrefixedKVCache) else None
         if self._beam is not None and T != 1:
             raise ValueError("a beam cache takes one token per row")
         decode = T == 1 and cache is not None and self._beam is None
         fused = decode and self._fused_decode_ok(B, collect_hidden)
         chain = decode and self._fused_decode_ok(B, collect_hidden, rows_in_lds=False) and self._chain_decode_ok(B)
         pend = None
-        if chain and self._relay_decode_ok(B, key_bias, n_keys_max):
+        if chain and type(cache) is KVCache and self._relay_decode_ok(B, key_bias, n_keys_max):
             x = self._relay_blocks(x, cache, past_len, key_bias, graph_pos, n_keys_max)
             blocks = ()
         else:
@@ -762,7 +929,7 @@ class OLMo(nn.Module):
             if collect_hidden:
                 hidden.append(x)
             if cache is not None:
-                kc, vc = cache.k[i], cache.v[i]
+                kc, vc = cache.layer(i)
             else:
                 kc, vc = self._scratch_cache(B, T)
             if chain:
@@ -808,7 +975,7 @@ class OLMo(nn.Module):
                  attention_bias: Optional[torch.Tensor] = None, max_steps: int = 10, beam_size: int = 1, per_node_beam_size: Optional[int] = None,
                  sampler=None, min_steps: Optional[int] = None, final_sequence_scorer=None,
                  constraints: Optional[list] = None, use_graph: bool = True, stop_at_eos: bool = True,
-                 seed: int = 0) -> OLMoGenerateOutput:
+                 seed: int = 0, prefix: Optional[SharedPrefix] = None) -> OLMoGenerateOutput:
         """``OLMo.generate`` (``olmo/model.py:1603-1728``).
 
         Beam size 1 without constraints, ``min_steps`` or a scorer is the captured greedy loop
@@ -819,13 +986,17 @@ class OLMo(nn.Module):
         ``max_steps`` and leaves the tokens as generated).  Anything else is ``olmo_amd.beam_search.BeamSearch``
         over a :class:`BeamKVCache`.  ``scores`` is the
         summed log-probability of the chosen tokens under the unfiltered distribution (passed through
-        ``final_sequence_scorer`` in a beam search)."""
+        ``final_sequence_scorer`` in a beam search).  ``prefix``: a prompt shared by the batch (:meth:`share_prefix`;
+        ``input_ids`` are what follows it), beam size 1 only."""
         if attention_bias is not None:  # olmo/model.py:1645-1657
             B, P = input_ids.shape
             assert attention_bias.dim() == 4 and tuple(attention_bias.shape[:2]) == (B, 1)
             assert P + max_steps <= attention_bias.shape[2] == attention_bias.shape[3]
         plain = beam_size == 1 and not constraints and not min_steps and final_sequence_scorer is None
         if not plain:
+            if prefix is not None or self.kv_cache is not None:
+                raise NotImplementedError("beam search and constraints keep one cache in the activation dtype: not with a shared "
+                                          "prefix or kv_cache='int8'")
             return self._generate_beam(input_ids, attention_mask, max_steps, beam_size, per_node_beam_size, sampler,
                                        min_steps, final_sequence_scorer, constraints, use_graph, attention_bias)
         from .generate import greedy_generate
@@ -838,7 +1009,7 @@ class OLMo(nn.Module):
         toks, scores = greedy_generate(self, input_ids, attention_mask, max_steps, use_graph=use_graph,
                                        eos_token_id=self.config.eos_token_id if stop_at_eos else None,
                                        return_scores=True, sampling=sampling, stop_when_all_ended=stop_at_eos,
-                                       attention_bias=attention_bias)
+                                       attention_bias=attention_bias, prefix=prefix)
         return OLMoGenerateOutput(token_ids=toks.unsqueeze(1), scores=scores.unsqueeze(1))
 
     def _generate_beam(self, input_ids, attention_mask, max_steps, beam_size, per_node_beam_size, sampler, min_steps,

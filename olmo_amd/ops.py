@@ -995,7 +995,7 @@ def qknorm_rope_kvwrite_q8(qkv, q_weight, k_weight, sin_tab, cos_tab, cache: KVQ
                            kcache: Optional[torch.Tensor] = None, vcache: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`qknorm_rope_kvwrite` into an 8-bit cache: returns q (normed + rotated) ``[B, T, H*hd]`` and writes codes and
     scales of the rotated k and of v.  float32 all the way to the codes (q: to its one rounding).  ``kcache`` /
-    ``vcache`` ``[B, Hkv, Lmax, hd]``, if given, receive the same rows unquantised."""
+    ``vcache`` ``[B, Hkv, L, hd]``, if given, receive the same rows unquantised."""
     _dev(qkv, q_weight, k_weight, sin_tab, cos_tab, kcache, vcache, past_len_dev, cache.k)
     _current(qkv)
     if qkv.shape[-1] != (H + 2 * Hkv) * hd or qkv.numel() != B * T * (H + 2 * Hkv) * hd:
@@ -1006,8 +1006,9 @@ def qknorm_rope_kvwrite_q8(qkv, q_weight, k_weight, sin_tab, cos_tab, cache: KVQ
         raise ValueError("kcache and vcache, q_weight and k_weight: both or neither")
     Lmax, n_pos = cache.k.shape[2], sin_tab.shape[0]
     if kcache is not None and (kcache.dtype != qkv.dtype or vcache.dtype != qkv.dtype or kcache.shape != vcache.shape
-                               or kcache.shape != (kcache.shape[0], Hkv, Lmax, hd) or kcache.shape[0] < B):
-        raise ValueError("kcache / vcache: [B, Hkv, Lmax, hd] of qkv's dtype and of the 8-bit cache's length expected")
+                               or kcache.dim() != 4 or kcache.shape[0] < B or kcache.shape[1] != Hkv or kcache.shape[3] != hd
+                               or (past_len_dev is None and past_len + T > kcache.shape[2])):
+        raise ValueError("kcache / vcache: [B, Hkv, L, hd] of qkv's dtype with room for the new rows expected")
     if q_weight is not None and (q_weight.dtype != qkv.dtype or k_weight.dtype != qkv.dtype or q_weight.numel() != H * hd
                                  or k_weight.numel() != Hkv * hd):
         raise ValueError("q_weight [H * hd] and k_weight [Hkv * hd] of qkv's dtype expected")
@@ -1020,7 +1021,8 @@ def qknorm_rope_kvwrite_q8(qkv, q_weight, k_weight, sin_tab, cos_tab, cache: KVQ
     if B * T:
         check("olmo355_qknorm_rope_kvwrite_q8",
               lib().olmo355_qknorm_rope_kvwrite_q8(_p(qkv), _p(q_weight), _p(k_weight), _p(sin_tab), _p(cos_tab), _p(q),
-                                                   *cache._args(), _p(kcache), _p(vcache), B, T, H, Hkv, hd, Lmax, n_pos, past_len,
+                                                   *cache._args(), _p(kcache), _p(vcache),
+                                                   kcache.shape[2] if kcache is not None else 0, B, T, H, Hkv, hd, Lmax, n_pos, past_len,
                                                    _p(past_len_dev), float(eps), _dt(qkv), _stream()))
     return q
 

@@ -12,12 +12,12 @@ def test_quantised_cache_and_shared_prefix_entries_refuse_without_launching():
     p = (ctypes.addressof(buf) + 15) & ~15
     EINVAL, EUNSUP = 1, 2
 
-    def write(qkv=p, qw=p, kw=p, kq=p, kc=None, vc=None, B=1, T=1, H=4, Hkv=2, hd=64, Lmax=8, n_pos=8, past=0, dev=None, dt=1):
-        return h.olmo355_qknorm_rope_kvwrite_q8(qkv, qw, kw, p, p, p, kq, p, p, p, kc, vc, B, T, H, Hkv, hd, Lmax, n_pos, past, dev, 1e-6,
+    def write(qkv=p, qw=p, kw=p, kq=p, kc=None, vc=None, Lfull=0, B=1, T=1, H=4, Hkv=2, hd=64, Lmax=8, n_pos=8, past=0, dev=None, dt=1):
+        return h.olmo355_qknorm_rope_kvwrite_q8(qkv, qw, kw, p, p, p, kq, p, p, p, kc, vc, Lfull, B, T, H, Hkv, hd, Lmax, n_pos, past, dev, 1e-6,
                                                 dt, None)
 
     for bad in (dict(qkv=None), dict(kw=None), dict(kc=p), dict(kq=p + 4), dict(qkv=p + 2), dict(B=0), dict(T=0), dict(H=3), dict(past=8),
-                dict(past=-1), dict(T=9), dict(n_pos=0), dict(past=2**31 - 1)):
+                dict(past=-1), dict(T=9), dict(n_pos=0), dict(past=2**31 - 1), dict(kc=p, vc=p, Lfull=3, past=3), dict(kc=p, vc=p)):
         assert write(**bad) == EINVAL, bad
     for bad in (dict(hd=96), dict(dt=3), dict(dev=p, T=2), dict(H=256, Hkv=256, hd=128)):
         assert write(**bad) == EUNSUP, bad

@@ -81,7 +81,7 @@ def test_write_and_read_back(dev, dtype, B, T, past, H, Hkv, hd, norm):
         t.fill_(77)
     for t in (c.k_scale, c.v_scale):
         t.fill_(-5.0)
-    kf, vf = (torch.full((B, Hkv, n, hd), 9.0, dtype=dtype, device=dev) for _ in range(2))
+    kf, vf = (torch.full((B, Hkv, n - 2, hd), 9.0, dtype=dtype, device=dev) for _ in range(2))  # of a length of their own
     d = lambda t: None if t is None else t.to(dev)
     q = ops.qknorm_rope_kvwrite_q8(d(qkv), d(qw), d(kw), d(sin), d(cos), c, B, T, H, Hkv, hd, past, eps, kcache=kf, vcache=vf)
     h = half(dtype)
@@ -324,6 +324,7 @@ def test_refusals(dev):
     w()
     pos = torch.zeros(1, dtype=torch.int32, device=dev)
     for bad in (dict(past_len=n), dict(past_len=-1), dict(k_weight=None), dict(kcache=torch.zeros(B, Hkv, n, hd, device=dev)),
+                dict(past_len=3, kcache=qkv.new_zeros(B, Hkv, 3, hd), vcache=qkv.new_zeros(B, Hkv, 3, hd)),
                 dict(Hkv=4), dict(H=5), dict(B=3), dict(q_weight=qw.float()), dict(sin_tab=sin.double()), dict(past_len_dev=pos.long()),
                 dict(qkv=qkv.repeat(1, 2, 1), T=2, past_len_dev=pos), dict(qkv=qkv.repeat(1, 1, 2)[..., ::2])):
         with pytest.raises((ValueError, TypeError)):
