@@ -960,6 +960,7 @@ class KVQ8:
             raise TypeError("KVQ8: int8 codes [B, Hkv, Lmax, hd] expected")
         if any(t.dtype != torch.float32 or t.shape != self.k.shape[:3] for t in (self.k_scale, self.v_scale)):
             raise TypeError("KVQ8: float32 scales [B, Hkv, Lmax] expected")
+        object.__setattr__(self, "dims", tuple(self.k.shape))  # looked at once, not per call
 
     @classmethod
     def empty(cls, B: int, Hkv: int, Lmax: int, hd: int, device) -> "KVQ8":
@@ -970,11 +971,29 @@ class KVQ8:
     def _args(self):
         return self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr()
 
+    def _fits(self, B: int, Hkv: int, hd: int) -> None:
+        b, h, _, d = self.dims
+        if b < B or h != Hkv or d != hd:
+            raise ValueError(f"cache shape {self.dims} does not fit B={B} Hkv={Hkv} hd={hd}")
 
-def _current(t: torch.Tensor) -> None:
-    """Launches go to the current device's stream."""
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"tensors on {t.device}, but the current device is cuda:{torch.cuda.current_device()}")
+
+def _launch_device(*ts: Optional[torch.Tensor]) -> int:
+    """:func:`_dev`, and the tensors' device is the current one, whose stream the launch goes to; its index."""
+    dev = -1
+    for t in ts:
+        if t is None:
+            continue
+        d = t.get_device()
+        if d < 0 or (dev >= 0 and d != dev) or not t.is_contiguous():
+            _dev(*ts)  # says what is wrong
+        dev = d
+    if dev != torch.cuda.current_device():
+        raise ValueError(f"tensors on cuda:{dev}, but the current device is cuda:{torch.cuda.current_device()}")
+    return dev
+
+
+def _stream_of(dev: int) -> int:
+    return _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
 
 
 def _past_dev_ok(past_len_dev: Optional[torch.Tensor], T: int) -> None:
@@ -990,40 +1009,49 @@ def _key_bias_stride(key_bias: Optional[torch.Tensor], B: int, n: int) -> int:
     return key_bias.shape[1]
 
 
+def _check_lengths(fn: str, st: int, what: str, ws: Optional[torch.Tensor] = None, need: int = 0) -> None:
+    """A refusal of the library in this module's words: of its numbers only lengths are left unchecked up to the call."""
+    if st == 1 and ws is not None and _nbytes(ws) < need:
+        raise ValueError(f"{fn}: attention workspace too small ({_nbytes(ws)} of {need} bytes)")
+    if st == 1 and what:
+        raise ValueError(f"{fn}: {what} (or a tensor that does not start on 16 bytes)")
+    check(fn, st)
+
+
 def qknorm_rope_kvwrite_q8(qkv, q_weight, k_weight, sin_tab, cos_tab, cache: KVQ8, B: int, T: int, H: int, Hkv: int, hd: int,
                            past_len: int, eps: float, past_len_dev: Optional[torch.Tensor] = None,
                            kcache: Optional[torch.Tensor] = None, vcache: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`qknorm_rope_kvwrite` into an 8-bit cache: returns q (normed + rotated) ``[B, T, H*hd]`` and writes codes and
     scales of the rotated k and of v.  float32 all the way to the codes (q: to its one rounding).  ``kcache`` /
-    ``vcache`` ``[B, Hkv, L, hd]``, if given, receive the same rows unquantised."""
-    _dev(qkv, q_weight, k_weight, sin_tab, cos_tab, kcache, vcache, past_len_dev, cache.k)
-    _current(qkv)
+    ``vcache`` ``[B, Hkv, L, hd]``, if given, receive the same rows unquantised.  Tensors start on 16 bytes."""
+    dev = _launch_device(qkv, q_weight, k_weight, sin_tab, cos_tab, kcache, vcache, past_len_dev, cache.k)
+    dtype = qkv.dtype
     if qkv.shape[-1] != (H + 2 * Hkv) * hd or qkv.numel() != B * T * (H + 2 * Hkv) * hd:
         raise ValueError("qkv shape mismatch")
-    if cache.k.shape[0] < B or cache.k.shape[1] != Hkv or cache.k.shape[3] != hd:
-        raise ValueError(f"cache shape {tuple(cache.k.shape)} does not fit B={B} Hkv={Hkv} hd={hd}")
+    cache._fits(B, Hkv, hd)
     if (kcache is None) != (vcache is None) or (q_weight is None) != (k_weight is None):
         raise ValueError("kcache and vcache, q_weight and k_weight: both or neither")
-    Lmax, n_pos = cache.k.shape[2], sin_tab.shape[0]
-    if kcache is not None and (kcache.dtype != qkv.dtype or vcache.dtype != qkv.dtype or kcache.shape != vcache.shape
-                               or kcache.dim() != 4 or kcache.shape[0] < B or kcache.shape[1] != Hkv or kcache.shape[3] != hd
-                               or (past_len_dev is None and past_len + T > kcache.shape[2])):
-        raise ValueError("kcache / vcache: [B, Hkv, L, hd] of qkv's dtype with room for the new rows expected")
-    if q_weight is not None and (q_weight.dtype != qkv.dtype or k_weight.dtype != qkv.dtype or q_weight.numel() != H * hd
+    Lfull = 0
+    if kcache is not None:
+        Lfull = kcache.shape[2] if kcache.dim() == 4 else 0
+        if (kcache.dtype != dtype or vcache.dtype != dtype or kcache.shape != vcache.shape or not Lfull or kcache.shape[0] < B
+                or kcache.shape[1] != Hkv or kcache.shape[3] != hd):
+            raise ValueError("kcache / vcache: [B, Hkv, L, hd] of qkv's dtype expected")
+    if q_weight is not None and (q_weight.dtype != dtype or k_weight.dtype != dtype or q_weight.numel() != H * hd
                                  or k_weight.numel() != Hkv * hd):
         raise ValueError("q_weight [H * hd] and k_weight [Hkv * hd] of qkv's dtype expected")
-    if sin_tab.dtype != torch.float32 or cos_tab.dtype != torch.float32 or sin_tab.shape != cos_tab.shape or sin_tab.shape[-1] != hd:
+    n_pos = sin_tab.shape[0]
+    if sin_tab.dtype != torch.float32 or cos_tab.dtype != torch.float32 or sin_tab.shape != cos_tab.shape or sin_tab.numel() != n_pos * hd:
         raise ValueError("sin/cos tables must be float32 [n_pos, hd]")
     _past_dev_ok(past_len_dev, T)
-    if past_len_dev is None and not 0 <= past_len <= min(Lmax, n_pos) - T:
-        raise ValueError(f"rows {past_len} .. {past_len + T - 1} outside the cache ({Lmax}) or the rotary table ({n_pos})")
-    q = torch.empty(B, T, H * hd, dtype=qkv.dtype, device=qkv.device)
+    q = qkv.new_empty((B, T, H * hd))
     if B * T:
-        check("olmo355_qknorm_rope_kvwrite_q8",
-              lib().olmo355_qknorm_rope_kvwrite_q8(_p(qkv), _p(q_weight), _p(k_weight), _p(sin_tab), _p(cos_tab), _p(q),
-                                                   *cache._args(), _p(kcache), _p(vcache),
-                                                   kcache.shape[2] if kcache is not None else 0, B, T, H, Hkv, hd, Lmax, n_pos, past_len,
-                                                   _p(past_len_dev), float(eps), _dt(qkv), _stream()))
+        st = lib().olmo355_qknorm_rope_kvwrite_q8(_p(qkv), _p(q_weight), _p(k_weight), _p(sin_tab), _p(cos_tab), _p(q), *cache._args(),
+                                                  _p(kcache), _p(vcache), Lfull, B, T, H, Hkv, hd, cache.dims[2], n_pos, past_len,
+                                                  _p(past_len_dev), eps, _dt(qkv), _stream_of(dev))
+        if st:
+            _check_lengths("olmo355_qknorm_rope_kvwrite_q8", st, f"rows {past_len} .. {past_len + T - 1} outside the cache "
+                           f"({cache.dims[2]}), the rotary table ({n_pos}) or kcache ({Lfull or 'none'}), or heads that do not divide")
     return q
 
 
@@ -1031,24 +1059,25 @@ def kv_read_q8(cache: KVQ8, start: int, n: int, dtype: torch.dtype,
                out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Rows ``start .. start + n - 1`` of an 8-bit cache as values (``code * scale``, one rounding to ``dtype``): new
     ``(k, v)`` of shape ``[B, Hkv, n, hd]``, or into the same rows of ``out``, a pair of caches ``[B, Hkv, L, hd]``."""
-    B, Hkv, Lmax, hd = cache.k.shape
-    _current(cache.k)
+    B, Hkv, Lmax, hd = cache.dims
     if start < 0 or n < 0 or start + n > Lmax:
         raise ValueError(f"rows {start} .. {start + n - 1} outside the cache of {Lmax}")
     if out is None:
-        kv = torch.empty(2, B, Hkv, n, hd, dtype=dtype, device=cache.k.device)
-        k, v, at = kv[0], kv[1], 0
+        dev = _launch_device(cache.k)
+        k, v = cache.k.new_empty((B, Hkv, n, hd), dtype=dtype), cache.k.new_empty((B, Hkv, n, hd), dtype=dtype)
+        L, at = n, 0
     else:
         (k, v), at = out, start
-        _dev(k, v, cache.k)
+        dev = _launch_device(k, v, cache.k)
         if k.dtype != dtype or v.dtype != dtype or k.shape != v.shape or k.dim() != 4 or (k.shape[0], k.shape[1], k.shape[3]) != (B, Hkv, hd):
             raise ValueError(f"out: two caches [{B}, {Hkv}, L, {hd}] of {dtype} expected")
-        if k.shape[2] < start + n:
+        L = k.shape[2]
+        if L < start + n:
             raise ValueError("out is too short")
     dt = _dt(k)
     if n and B:
         check("olmo355_kv_read_q8",
-              lib().olmo355_kv_read_q8(*cache._args(), _p(k), _p(v), B, Hkv, hd, Lmax, start, n, k.shape[2], at, dt, _stream()))
+              lib().olmo355_kv_read_q8(*cache._args(), _p(k), _p(v), B, Hkv, hd, Lmax, start, n, L, at, dt, _stream_of(dev)))
     return k, v
 
 
@@ -1061,23 +1090,18 @@ def attn_decode_q8(q, cache: KVQ8, ws: torch.Tensor, B: int, H: int, Hkv: int, h
                    key_bias: Optional[torch.Tensor] = None, past_len_dev: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`attn_decode` over an 8-bit cache: one query per sequence, keys ``0 .. past_len``; ``ws`` from
     :func:`attn_decode_q8_workspace` (one per stream: overlapping calls must not share it)."""
-    _dev(q, cache.k, ws, key_bias, past_len_dev)
-    _current(q)
+    dev = _launch_device(q, cache.k, ws, key_bias, past_len_dev)
     if q.numel() != B * H * hd:
         raise ValueError("q shape mismatch")
-    if cache.k.shape[0] < B or cache.k.shape[1] != Hkv or cache.k.shape[3] != hd:
-        raise ValueError(f"cache shape {tuple(cache.k.shape)} does not fit B={B} Hkv={Hkv} hd={hd}")
+    cache._fits(B, Hkv, hd)
     _past_dev_ok(past_len_dev, 1)
-    Lmax = cache.k.shape[2]
-    if not 0 < n_keys_max <= Lmax or (past_len_dev is None and not 0 <= past_len < n_keys_max):
-        raise ValueError(f"past_len {past_len}, n_keys_max {n_keys_max} do not fit a cache of {Lmax}")
     stride = _key_bias_stride(key_bias, B, n_keys_max)
-    if _nbytes(ws) < int(lib().olmo355_attn_decode_q8_workspace_bytes(B, H, Hkv, hd, n_keys_max)):
-        raise ValueError("attention workspace too small")
-    out = torch.empty(B, 1, H * hd, dtype=q.dtype, device=q.device)
-    check("olmo355_attn_decode_q8",
-          lib().olmo355_attn_decode_q8(_p(q), *cache._args(), _p(key_bias), _p(out), _p(ws), _nbytes(ws), B, H, Hkv, hd, Lmax,
-                                       past_len, _p(past_len_dev), n_keys_max, stride, _dt(q), _stream()))
+    out = q.new_empty((B, 1, H * hd))
+    st = lib().olmo355_attn_decode_q8(_p(q), *cache._args(), _p(key_bias), _p(out), _p(ws), _nbytes(ws), B, H, Hkv, hd, cache.dims[2],
+                                      past_len, _p(past_len_dev), n_keys_max, stride, _dt(q), _stream_of(dev)) if B else 0
+    if st:
+        _check_lengths("olmo355_attn_decode_q8", st, f"past_len {past_len}, n_keys_max {n_keys_max} do not fit a cache of {cache.dims[2]}, "
+                       "or heads that do not divide", ws, int(lib().olmo355_attn_decode_q8_workspace_bytes(B, H, Hkv, hd, n_keys_max)))
     return out
 
 
@@ -1097,32 +1121,27 @@ def attn_shared_prefix(q, kprefix, vprefix, kcache, vcache, ws: torch.Tensor, B:
     prefix_len - 1`` of ``kprefix`` / ``vprefix`` (``[Hkv, P, hd]``, held and read once), then rows ``0 .. past_len + t``
     of the sequence's own caches ``[B, Hkv, Lmax, hd]`` (already written).  ``key_bias`` ``[B, n]`` is for the own rows; a
     masked one weighs nothing.  ``ws`` from :func:`attn_shared_prefix_workspace` (one per stream)."""
-    _dev(q, kprefix, vprefix, kcache, vcache, ws, key_bias, past_len_dev)
-    _current(q)
+    dev = _launch_device(q, kprefix, vprefix, kcache, vcache, ws, key_bias, past_len_dev)
     if q.numel() != B * T * H * hd:
         raise ValueError("q shape mismatch")
-    if any(t.dtype != q.dtype for t in (kprefix, vprefix, kcache, vcache)):
+    dtype = q.dtype
+    if kprefix.dtype != dtype or vprefix.dtype != dtype or kcache.dtype != dtype or vcache.dtype != dtype:
         raise TypeError("prefix and caches must have q's dtype")
-    if kprefix.dim() != 3 or kprefix.shape != vprefix.shape or kprefix.shape[0] != Hkv or kprefix.shape[2] != hd:
-        raise ValueError(f"prefix shape {tuple(kprefix.shape)} is not [Hkv={Hkv}, P, hd={hd}]")
-    if kcache.dim() != 4 or kcache.shape != vcache.shape or kcache.shape[0] < B or kcache.shape[1] != Hkv or kcache.shape[3] != hd:
-        raise ValueError(f"cache shape {tuple(kcache.shape)} does not fit B={B} Hkv={Hkv} hd={hd}")
-    if not 0 < prefix_len <= kprefix.shape[1]:
-        raise ValueError(f"prefix_len {prefix_len} outside 1 .. {kprefix.shape[1]} (without a prefix: attn_prefill / attn_decode)")
+    ps, cs = kprefix.shape, kcache.shape
+    if len(ps) != 3 or ps != vprefix.shape or ps[0] != Hkv or ps[2] != hd:
+        raise ValueError(f"prefix shape {tuple(ps)} is not [Hkv={Hkv}, P, hd={hd}]")
+    if len(cs) != 4 or cs != vcache.shape or cs[0] < B or cs[1] != Hkv or cs[3] != hd:
+        raise ValueError(f"cache shape {tuple(cs)} does not fit B={B} Hkv={Hkv} hd={hd}")
     _past_dev_ok(past_len_dev, T)
-    if n_keys_max > kcache.shape[2] or n_keys_max < T or (past_len_dev is None and not 0 <= past_len <= n_keys_max - T):
-        raise ValueError(f"past_len {past_len} + {T} new tokens, n_keys_max {n_keys_max} do not fit a cache of {kcache.shape[2]}")
     stride = _key_bias_stride(key_bias, B, n_keys_max)
-    dt = _dt(q)
-    out = torch.empty(B, T, H * hd, dtype=q.dtype, device=q.device)
-    if not out.numel():
-        return out
-    if _nbytes(ws) < int(lib().olmo355_attn_shared_prefix_workspace_bytes(B, T, H, Hkv, hd, prefix_len, n_keys_max, dt)):
-        raise ValueError("attention workspace too small")
-    check("olmo355_attn_shared_prefix",
-          lib().olmo355_attn_shared_prefix(_p(q), _p(kprefix), _p(vprefix), _p(kcache), _p(vcache), _p(key_bias), _p(out), _p(ws),
-                                           _nbytes(ws), B, T, H, Hkv, hd, prefix_len, kprefix.shape[1], kcache.shape[2], past_len,
-                                           _p(past_len_dev), n_keys_max, stride, dt, _stream()))
+    out = q.new_empty((B, T, H * hd))
+    st = lib().olmo355_attn_shared_prefix(_p(q), _p(kprefix), _p(vprefix), _p(kcache), _p(vcache), _p(key_bias), _p(out), _p(ws),
+                                          _nbytes(ws), B, T, H, Hkv, hd, prefix_len, ps[1], cs[2], past_len, _p(past_len_dev), n_keys_max,
+                                          stride, _dt(q), _stream_of(dev)) if B * T else 0
+    if st:
+        _check_lengths("olmo355_attn_shared_prefix", st, f"prefix_len {prefix_len} (at least 1) of {ps[1]}, past_len {past_len} + {T} new "
+                       f"tokens, n_keys_max {n_keys_max} do not fit a cache of {cs[2]}, or heads that do not divide", ws,
+                       int(lib().olmo355_attn_shared_prefix_workspace_bytes(B, T, H, Hkv, hd, prefix_len, n_keys_max, _dt(q))))
     return out
 
 

@@ -351,7 +351,5 @@ def test_refusals(dev):
             a(**bad)
     # a buffer that does not start on 16 bytes
     odd = torch.zeros(B * H * hd + 1, dtype=torch.bfloat16, device=dev)[1:].view(B, 1, H * hd)
-    from olmo_amd._lib import Olmo355Error
-
-    with pytest.raises(Olmo355Error):
+    with pytest.raises(ValueError):
         a(q=odd)
