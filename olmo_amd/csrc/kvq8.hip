@@ -11,25 +11,37 @@
 
 namespace {
 
-// eight activations as floats, and back (16 bytes of a 16-bit type, 32 of fp32)
+// eight activations: as they lie in memory (16 bytes of a 16-bit type, 32 of fp32), as floats, and back
 template <int DT>
-__device__ __forceinline__ void ld8f(const void* p, int64_t e, float (&f)[8]) {
-  if constexpr (DT == O355_F32) {
-    const f32x4 a = reinterpret_cast<const f32x4*>((const float*)p + e)[0], b = reinterpret_cast<const f32x4*>((const float*)p + e)[1];
+struct Raw8 {
+  u32x4 w[DT == O355_F32 ? 2 : 1];
+  __device__ __forceinline__ void ld(const void* p, int64_t e) {
+    if constexpr (DT == O355_F32) {
+      w[0] = reinterpret_cast<const u32x4*>((const float*)p + e)[0], w[1] = reinterpret_cast<const u32x4*>((const float*)p + e)[1];
+    } else {
+      w[0] = *reinterpret_cast<const u32x4*>((const uint16_t*)p + e);
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    if constexpr (DT == O355_F32) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = a[i], f[4 + i] = b[i];
-  } else {
-    const u32x4 w = *reinterpret_cast<const u32x4*>((const uint16_t*)p + e);
-    if constexpr (DT == O355_BF16) {
-      unpack8(w, f);
+      for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(w[0][i]), f[4 + i] = __uint_as_float(w[1][i]);
+    } else if constexpr (DT == O355_BF16) {
+      unpack8(w[0], f);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const f16x2 h = __builtin_bit_cast(f16x2, (uint32_t)w[i]);
+        const f16x2 h = __builtin_bit_cast(f16x2, (uint32_t)w[0][i]);
         f[2 * i] = (float)h[0], f[2 * i + 1] = (float)h[1];
       }
     }
   }
+};
+template <int DT>
+__device__ __forceinline__ void ld8f(const void* p, int64_t e, float (&f)[8]) {
+  Raw8<DT> r;
+  r.ld(p, e);
+  r.get(f);
 }
 template <int DT>
 __device__ __forceinline__ void st8f(void* p, int64_t e, const float (&f)[8]) {
@@ -46,37 +58,40 @@ __device__ __forceinline__ void st8f(void* p, int64_t e, const float (&f)[8]) {
 }
 
 // ---- write ----------------------------------------------------------------------------------------------------
-// Grid (token row, part): part 0 normalises and rotates q, part 1 k, part 2 takes v: the sum of squares of q and of k are
-// over the whole width (olmo/model.py:603-605), so a workgroup needs one of them and reads nothing twice.  A thread owns
-// channels j .. j + 7 of the first half of a head and the 8 they rotate with; hd / 16 neighbouring lanes hold a head, whose
-// maximum is a few register exchanges.  fp32 from the input to the code (q: to its one rounding).
-template <int DT, int HD, int CPT>
+// Grid (token rows, part): part 0 normalises and rotates q, part 1 k, part 2 takes v: the sum of squares of q and of k are
+// over the whole width (olmo/model.py:603-605), so whoever takes a part needs one of them and reads nothing twice.  A row's
+// part is one wave's (WPR 1: no barrier, four tokens to a workgroup) or a workgroup's (WPR 4).  A lane owns channels
+// j .. j + 7 of the first half of a head and the 8 they rotate with, CPT such pairs, which stay in registers as they were
+// loaded; hd / 16 neighbouring lanes hold a head, whose maximum is a few register exchanges.  fp32 from the input to the
+// code (q: to its one rounding).
+template <int DT, int HD, int CPT, int WPR>
 __global__ __launch_bounds__(256) void kv_write_q8_kernel(const void* __restrict__ qkv, const void* __restrict__ qw,
                                                           const void* __restrict__ kw, const float* __restrict__ sin_t,
                                                           const float* __restrict__ cos_t, void* __restrict__ q_out,
                                                           int8_t* __restrict__ kq, int8_t* __restrict__ vq, float* __restrict__ ks,
-                                                          float* __restrict__ vs, void* __restrict__ kc, void* __restrict__ vc, int Lfull, int T,
-                                                          int H, int Hkv, int Lmax, int n_pos, int past_len,
+                                                          float* __restrict__ vs, void* __restrict__ kc, void* __restrict__ vc, int Lfull,
+                                                          uint32_t rows, uint32_t T, int H, int Hkv, int Lmax, int n_pos, int past_len,
                                                           const int32_t* __restrict__ past_dev, float eps) {
-  constexpr int CPH = HD / 16, HALF = HD / 2;
+  constexpr int CPH = HD / 16, HALF = HD / 2, LANES = 64 * WPR;
   __shared__ float red[16];
-  const int part = blockIdx.y;
-  const int64_t row = blockIdx.x;
-  const int b = (int)(row / T), t = (int)(row - (int64_t)b * T);
+  const int part = blockIdx.y, me = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
+  const uint32_t row = WPR == 1 ? blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x;
+  if (row >= rows) return;  // WPR 1: whole waves
+  const uint32_t b = row / T, t = row - b * T;
   const int dq = H * HD, dk = Hkv * HD;
-  const int pos = (past_dev ? *past_dev : past_len) + t;
+  const int pos = (past_dev ? *past_dev : past_len) + (int)t;
   if (pos < 0 || pos >= Lmax || pos >= n_pos) return;  // a device-side position outside the cache: write nothing
   const int heads = part == 0 ? H : Hkv, n = heads * CPH;
-  const int64_t in = row * (dq + 2 * dk) + (part == 0 ? 0 : part == 1 ? dq : dq + dk);
+  const int64_t in = (int64_t)row * (dq + 2 * dk) + (part == 0 ? 0 : part == 1 ? dq : dq + dk);
   const void* w = part == 0 ? qw : part == 1 ? kw : nullptr;
-  float x1[CPT][8], x2[CPT][8];
+  Raw8<DT> x1[CPT], x2[CPT];
 #pragma unroll
   for (int i = 0; i < CPT; ++i) {
-    const int c = threadIdx.x + i * 256;
+    const int c = me + i * LANES;
     if (c < n) {
       const int64_t e = in + (c / CPH) * HD + (c % CPH) * 8;
-      ld8f<DT>(qkv, e, x1[i]);
-      ld8f<DT>(qkv, e + HALF, x2[i]);
+      x1[i].ld(qkv, e);
+      x2[i].ld(qkv, e + HALF);
     }
   }
   float rstd = 1.f;
@@ -84,55 +99,62 @@ __global__ __launch_bounds__(256) void kv_write_q8_kernel(const void* __restrict
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < CPT; ++i)
-      if (threadIdx.x + i * 256 < n) {
+      if (me + i * LANES < n) {
+        float a[8], bb[8];
+        x1[i].get(a), x2[i].get(bb);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss += x1[i][e] * x1[i][e] + x2[i][e] * x2[i][e];
+        for (int e = 0; e < 8; ++e) ss += a[e] * a[e] + bb[e] * bb[e];
       }
-    rstd = 1.f / sqrtf(block_sum(ss, red) / (float)(heads * HD) + eps);
+    if constexpr (WPR == 1) ss = wave_sum(ss);
+    else ss = block_sum(ss, red);
+    rstd = 1.f / sqrtf(ss / (float)(heads * HD) + eps);
   }
   const float* sn = sin_t + (int64_t)pos * HD;
   const float* cs = cos_t + (int64_t)pos * HD;
+  const int j = (me % CPH) * 8;  // LANES is a multiple of CPH: the same channels of a head in every pair
+  float c1[8], c2[8], s1[8], s2[8];
+  if (part < 2) ld8f<O355_F32>(cs, j, c1), ld8f<O355_F32>(cs, j + HALF, c2), ld8f<O355_F32>(sn, j, s1), ld8f<O355_F32>(sn, j + HALF, s2);
 #pragma unroll
   for (int i = 0; i < CPT; ++i) {
-    const int c = threadIdx.x + i * 256;
+    const int c = me + i * LANES;
     if (c >= n) break;  // the lanes of a head leave together
-    const int h = c / CPH, j = (c % CPH) * 8;
+    const int h = c / CPH;
+    float a[8], bb[8];
+    x1[i].get(a), x2[i].get(bb);
     if (w) {
       float w1[8], w2[8];
       ld8f<DT>(w, h * HD + j, w1);
       ld8f<DT>(w, h * HD + j + HALF, w2);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x1[i][e] = x1[i][e] * rstd * w1[e], x2[i][e] = x2[i][e] * rstd * w2[e];
+      for (int e = 0; e < 8; ++e) a[e] = a[e] * rstd * w1[e], bb[e] = bb[e] * rstd * w2[e];
     }
     if (part < 2) {
-      float c1[8], c2[8], s1[8], s2[8];
-      ld8f<O355_F32>(cs, j, c1), ld8f<O355_F32>(cs, j + HALF, c2), ld8f<O355_F32>(sn, j, s1), ld8f<O355_F32>(sn, j + HALF, s2);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float a = x1[i][e], bb = x2[i][e];
-        x1[i][e] = a * c1[e] - bb * s1[e];
-        x2[i][e] = bb * c2[e] + a * s2[e];
+        const float u = a[e], v = bb[e];
+        a[e] = u * c1[e] - v * s1[e];
+        bb[e] = v * c2[e] + u * s2[e];
       }
     }
     if (part == 0) {
-      st8f<DT>(q_out, row * dq + h * HD + j, x1[i]);
-      st8f<DT>(q_out, row * dq + h * HD + j + HALF, x2[i]);
+      st8f<DT>(q_out, (int64_t)row * dq + h * HD + j, a);
+      st8f<DT>(q_out, (int64_t)row * dq + h * HD + j + HALF, bb);
       continue;
     }
-    const int64_t at = ((int64_t)b * Hkv + h) * Lmax + pos;
+    const int64_t bh = (int64_t)b * Hkv + h, at = bh * Lmax + pos;
     if (kc && pos < Lfull) {  // the row as the unquantised cache would hold it
       void* full = part == 1 ? kc : vc;
-      const int64_t e = (((int64_t)b * Hkv + h) * Lfull + pos) * HD + j;
-      st8f<DT>(full, e, x1[i]);
-      st8f<DT>(full, e + HALF, x2[i]);
+      const int64_t e = (bh * Lfull + pos) * HD + j;
+      st8f<DT>(full, e, a);
+      st8f<DT>(full, e + HALF, bb);
     }
     float amax = 0.f;
     bool finite = true;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float a = fabsf(x1[i][e]), bb = fabsf(x2[i][e]);
-      finite = finite && a <= 3.4028234663852886e38f && bb <= 3.4028234663852886e38f;
-      amax = fmaxf(amax, fmaxf(a, bb));
+      const float u = fabsf(a[e]), v = fabsf(bb[e]);
+      finite = finite && u <= 3.4028234663852886e38f && v <= 3.4028234663852886e38f;
+      amax = fmaxf(amax, fmaxf(u, v));
     }
     if (!finite) amax = INFINITY;
     amax = fmaxf(amax, dpp_lane<0xB1>(amax));                          // quad_perm [1,0,3,2]
@@ -145,8 +167,8 @@ __global__ __launch_bounds__(256) void kv_write_q8_kernel(const void* __restrict
     u32x2 p1, p2;
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
-      p1[g] = code(x1[i][4 * g]) | code(x1[i][4 * g + 1]) << 8 | code(x1[i][4 * g + 2]) << 16 | code(x1[i][4 * g + 3]) << 24;
-      p2[g] = code(x2[i][4 * g]) | code(x2[i][4 * g + 1]) << 8 | code(x2[i][4 * g + 2]) << 16 | code(x2[i][4 * g + 3]) << 24;
+      p1[g] = code(a[4 * g]) | code(a[4 * g + 1]) << 8 | code(a[4 * g + 2]) << 16 | code(a[4 * g + 3]) << 24;
+      p2[g] = code(bb[4 * g]) | code(bb[4 * g + 1]) << 8 | code(bb[4 * g + 2]) << 16 | code(bb[4 * g + 3]) << 24;
     }
     int8_t* codes = part == 1 ? kq : vq;
     *reinterpret_cast<u32x2*>(codes + at * HD + j) = p1;
@@ -269,15 +291,26 @@ extern "C" int olmo355_qknorm_rope_kvwrite_q8(const void* qkv, const void* qw, c
   const int64_t chunks = (int64_t)H * hd / 16;
   if (chunks > 1024 || (int64_t)B * T > 0x7fffffff) return O355_EUNSUPPORTED;
   hipStream_t s = as_stream(stream);
-  const dim3 grid((unsigned)((int64_t)B * T), 3);
-#define WRITE(DTv, HDv, CPT)                                                                                                      \
-  hipLaunchKernelGGL((kv_write_q8_kernel<DTv, HDv, CPT>), grid, dim3(256), 0, s, qkv, qw, kw, sin_tab, cos_tab, q_out, kq, vq,    \
-                     kscale, vscale, kcache, vcache, Lfull, T, H, Hkv, Lmax, n_pos, past_len, past_len_dev, eps)
-#define WRITE_CPT(DTv, HDv)                  \
-  do {                                       \
-    if (chunks <= 256) WRITE(DTv, HDv, 1);   \
-    else if (chunks <= 512) WRITE(DTv, HDv, 2); \
-    else WRITE(DTv, HDv, 4);                 \
+  const uint32_t rows = (uint32_t)B * T;
+  // Few rows: a workgroup to a row's part, whose loads all go out at once (32 heads of 128, 1 row 4.8 us against 6.5 with a wave
+  // to it, 2048 rows 20.6 against 21.3); many rows, or short ones: a wave (40 heads, 8168 rows 95 against 97-104; 40 / 8
+  // heads, 8192 rows 52 against 59; 8 heads of 32, 8000 rows 15.5 against 25: the count of workgroups is what that costs).
+  // 8168 rows of 40 heads: 4.4 TB/s of the 4.8 that a large copy reaches.
+#define WRITE(DTv, HDv, CPT, WPR)                                                                                                  \
+  hipLaunchKernelGGL((kv_write_q8_kernel<DTv, HDv, CPT, WPR>), dim3(WPR == 1 ? (rows + 3) / 4 : rows, 3), dim3(256), 0, s, qkv, qw, \
+                     kw, sin_tab, cos_tab, q_out, kq, vq, kscale, vscale, kcache, vcache, Lfull, rows, (uint32_t)T, H, Hkv, Lmax,   \
+                     n_pos, past_len, past_len_dev, eps)
+#define WRITE_CPT(DTv, HDv)                            \
+  do {                                                 \
+    if (rows < 4096 && chunks > 128) {                 \
+      if (chunks <= 256) WRITE(DTv, HDv, 1, 4);        \
+      else if (chunks <= 512) WRITE(DTv, HDv, 2, 4);   \
+      else WRITE(DTv, HDv, 4, 4);                      \
+    } else if (chunks <= 64) WRITE(DTv, HDv, 1, 1);    \
+    else if (chunks <= 128) WRITE(DTv, HDv, 2, 1);     \
+    else if (chunks <= 256) WRITE(DTv, HDv, 4, 1);     \
+    else if (chunks <= 512) WRITE(DTv, HDv, 8, 1);     \
+    else WRITE(DTv, HDv, 4, 4);                        \
   } while (0)
   Q8_SWITCH(dtype, hd, WRITE_CPT)
 #undef WRITE_CPT
