@@ -116,6 +116,26 @@ def test_write_and_read_back(dev, dtype, B, T, past, H, Hkv, hd, norm):
     assert ops.kv_read_q8(c, n, 0, dtype)[0].shape == (B, Hkv, 0, hd)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,T,H,Hkv,hd", [(2, 2051, 40, 8, 128), (1, 4097, 24, 24, 128), (1, 4100, 14, 2, 128), (3, 1400, 5, 5, 32),
+                                          (1, 4099, 72, 1, 128), (1, 4200, 32, 4, 64)])
+def test_write_many_rows(dev, dtype, B, T, H, Hkv, hd):
+    """The launch forms for many rows; the reference in 64 bits on the device."""
+    ops = _ops()
+    print("write_q8 rows", dtype, B, T, H, Hkv, hd, flush=True)
+    qkv, qw, kw, sin, cos = (t.to(dev) for t in write_case(dtype, B, T, H, Hkv, hd, True, T, seed=T))
+    (q8, qa), (k8, ka), v8 = write_ref(qkv, qw, kw, sin, cos, B, T, H, Hkv, hd, 0, 1e-6)
+    c = ops.KVQ8.empty(B, Hkv, T, hd, dev)
+    q = ops.qknorm_rope_kvwrite_q8(qkv, qw, kw, sin, cos, c, B, T, H, Hkv, hd, 0, 1e-6)
+    # a lane adds up to 16 * 16 squares here before the exchange: half of (256 + 6) * 2^-24 for the root, below 2^-16
+    rel = 2.0 ** -16
+    assert ((q.double().view(B, T, H, hd) - q8).abs() <= half(dtype) * q8.abs() + rel * qa + 2.0 ** -25).all()
+    for codes, scale, x, off in ((c.k, c.k_scale, k8, rel * ka), (c.v, c.v_scale, v8, torch.zeros_like(v8))):
+        x, off, s = x.transpose(1, 2), off.transpose(1, 2), scale.double()
+        assert ((s - x.abs().amax(-1) / 127).abs() <= 2.0 ** -23 * s + off.amax(-1) / 127).all()
+        assert ((codes.double() - x / s.unsqueeze(-1)).abs() <= 0.5 + 127 * 3 * 2.0 ** -24 + off / s.unsqueeze(-1)).all()
+
+
 def test_write_rows_of_zeros_tiny_huge_and_not_finite(dev):
     """Row maxima from nothing to the largest number; a row with an infinity or a NaN reads back as NaN, its neighbours
     are untouched by it."""
