@@ -26,13 +26,13 @@ PrefixPlan prefix_plan(int B, int T, int H, int Hkv, int P, int n_keys_max) {
   p.tiles_p = (int)((rows_p + 16 * p.rtp - 1) / (16 * p.rtp));
   p.tiles_o = (int)((rows_o + 16 * p.rto - 1) / (16 * p.rto));
   auto at_most = [](int64_t want, int64_t most) { return (int)(want < 1 ? 1 : want > most ? most : want); };
-  // Own keys: two waves per SIMD, at least two steps each.  Prefix: two workgroups per CU, at least 128 keys (a step per wave)
-  // each; a small own part's workgroups count among those two, so that all are resident at once (4 sequences, 32 heads,
-  // prefix 16384: 59 us with 512 + 32 workgroups, 52 with 480 + 32; 32 sequences with 512 own ones are better off with 512
-  // + 512, 34.7 us against 36.7).
-  p.splits_o = at_most(2048 / ((int64_t)B * Hkv * p.tiles_o), (n_keys_max + 63ll) / 64);
-  const int64_t own = ((int64_t)B * p.tiles_o * p.splits_o + 3) / 4 * Hkv;
-  p.splits_p = at_most((own <= 192 ? 512 - own : 512) / ((int64_t)Hkv * p.tiles_p), (P + 127ll) / 128);
+  // Own keys: a wave per SIMD, at least two steps each.  Prefix: what fills the rest of two workgroups per CU, at least 128
+  // keys (a step per wave) each, so that the launch takes whole rounds: 4 sequences, 32 heads, prefix 16384 59 us with 512 +
+  // 32 workgroups, 52 with 480 + 32; 32 sequences, prefix 4001, 35-37 with 512 + 512 or 256 + 512, 33 with 256 + 256.
+  // (The count of own keys is not looked at beyond that: a captured step is launched for as many as the cache holds.)
+  p.splits_o = at_most(1024 / ((int64_t)B * Hkv * p.tiles_o), (n_keys_max + 63ll) / 64);
+  const int64_t own = ((int64_t)B * p.tiles_o * p.splits_o + 3) / 4 * Hkv, room = 512 - own % 512;
+  p.splits_p = at_most((room < 192 ? room + 512 : room) / ((int64_t)Hkv * p.tiles_p), (P + 127ll) / 128);
   p.wgs_p = (int64_t)p.tiles_p * p.splits_p;
   p.own_waves = (int64_t)B * p.tiles_o * p.splits_o;
   p.wgs_o = (p.own_waves + 3) / 4;
