@@ -245,13 +245,18 @@ __global__ __launch_bounds__(256, 2) void attn_decode_q8_kernel(const void* __re
   });
 }
 
-// Runs of keys per (sequence, kv head, row tile): enough workgroups for two per CU, at least 128 keys each (one step per
-// wave).
+// Runs of keys per (sequence, kv head, row tile), at least 128 keys each (one step per wave). A round of one workgroup per CU,
+// no more, is best where it keeps the CUs busy: 4 x 4096 keys, 32 heads, 28.8 us with 256 workgroups, 29.4 with 512;
+// 1 x 4096 12.4 against 13.0; 8 x 2048 26.0 against 29.0; 32 x 1000, 8 kv heads, 13.9 against 17.6 (one run each, no merge).
+// Where the last round would leave a quarter of the CUs idle, long keys are cut finer: 9 x 4096, 32 heads, 74.6 us in
+// whole runs, 63.1 in 3; 13 x 8000, 10 kv heads, 72 in whole runs, 57 in 3. Up to 2048 keys that costs more than it brings
+// (5 x 2000, 32 heads, 19.0 in whole runs, 20.2 in 3). Never less with more keys: a workspace for n serves fewer.
 int decode_q8_splits(int B, int H, int Hkv, int n_keys_max) {
-  const int64_t units = (int64_t)B * Hkv * ((H / Hkv + 15) / 16);
-  const int most = (n_keys_max + 127) / 128;
-  const int64_t want = (512 + units - 1) / units;
-  return (int)(want < 1 ? 1 : want > most ? most : want);
+  const int64_t units = (int64_t)B * Hkv * ((H / Hkv + 15) / 16), cus = 256;
+  const int64_t whole = units < cus ? cus / units : 1, rounds = (units * whole + cus - 1) / cus;
+  const bool idle = 4 * units * whole <= 3 * rounds * cus && n_keys_max > 2048;
+  const int64_t fine = 4 * cus / units, want = idle && fine > whole ? fine : whole, most = (n_keys_max + 127) / 128;
+  return (int)(want > most ? most : want);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }

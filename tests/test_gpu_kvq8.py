@@ -227,7 +227,7 @@ def decode_ref(q, host, keys, H, Hkv, hd, bias, dtype):
 DECODE = [
     (1, 1, 1, 1, 32), (2, 2, 4, 2, 64), (1, 31, 3, 3, 128), (2, 32, 8, 8, 32), (1, 33, 16, 16, 128), (3, 127, 6, 2, 64),
     (2, 128, 40, 8, 128), (1, 129, 8, 1, 128), (2, 517, 34, 2, 32), (1, 2049, 32, 32, 128), (5, 700, 4, 4, 64),
-    (1, 4100, 48, 2, 128), (40, 300, 16, 16, 64), (70, 97, 32, 8, 32),
+    (1, 4100, 48, 2, 128), (40, 300, 16, 16, 64), (70, 97, 32, 8, 32), (33, 2100, 8, 8, 32), (17, 2051, 16, 8, 64), (32, 515, 8, 8, 64),
 ]
 
 
