@@ -322,7 +322,7 @@ int olmo355_kv_read_q8(const int8_t* kq, const int8_t* vq, const float* kscale, 
 /* olmo355_attn_decode over that form: one query per sequence, scores (q . codes) * kscale / sqrt(hd) + bias, masked keys
  * (bias <= -1e30) as there.  ws: olmo355_attn_decode_q8_workspace_bytes(...) bytes, 16-byte aligned (0: ws may be NULL);
  * nothing in it outlives the call, so it needs no clearing and serves any launch of at most its size that is ordered
- * with the others on one stream. */
+ * with the others on one stream.  The size for n_keys_max (and prefix_len, below) serves fewer as well. */
 int64_t olmo355_attn_decode_q8_workspace_bytes(int B, int H, int Hkv, int hd, int n_keys_max);
 int olmo355_attn_decode_q8(const void* q, const int8_t* kq, const int8_t* vq, const float* kscale, const float* vscale,
                            const float* key_bias, void* out, void* ws, int64_t ws_bytes, int B, int H, int Hkv, int hd,

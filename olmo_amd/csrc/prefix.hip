@@ -13,6 +13,7 @@ struct PrefixPlan {
   int rtp, rto;          // 16-row tiles per workgroup, prefix part and own part
   int tiles_p, tiles_o;  // row tiles per kv head (prefix) and per sequence and kv head (own)
   int splits_p, splits_o;
+  int most_p;              // splits_p for any fewer own keys (what a workspace has to hold)
   int64_t wgs_p, wgs_o;    // workgroups per kv head
   int64_t own_waves;       // waves of the own part per kv head
 };
@@ -33,6 +34,7 @@ PrefixPlan prefix_plan(int B, int T, int H, int Hkv, int P, int n_keys_max) {
   p.splits_o = at_most(1024 / ((int64_t)B * Hkv * p.tiles_o), (n_keys_max + 63ll) / 64);
   const int64_t own = ((int64_t)B * p.tiles_o * p.splits_o + 3) / 4 * Hkv, room = 512 - own % 512;
   p.splits_p = at_most((room < 192 ? room + 512 : room) / ((int64_t)Hkv * p.tiles_p), (P + 127ll) / 128);
+  p.most_p = at_most((192 + 511) / ((int64_t)Hkv * p.tiles_p), (P + 127ll) / 128);
   p.wgs_p = (int64_t)p.tiles_p * p.splits_p;
   p.own_waves = (int64_t)B * p.tiles_o * p.splits_o;
   p.wgs_o = (p.own_waves + 3) / 4;
@@ -426,7 +428,7 @@ extern "C" int64_t olmo355_attn_shared_prefix_workspace_bytes(int B, int T, int 
   if (const int parts = prefix_chain_parts(B, T, H, Hkv, hd, prefix_len, n_keys_max, dtype))
     return parts == 1 ? 0 : 4 * rows_parts_floats((int64_t)B * T * H, hd, parts);
   const PrefixPlan p = prefix_plan(B, T, H, Hkv, prefix_len, n_keys_max);
-  return 4 * rows_parts_floats((int64_t)B * T * H, hd, p.splits_p + p.splits_o);
+  return 4 * rows_parts_floats((int64_t)B * T * H, hd, p.most_p + p.splits_o);
 }
 
 extern "C" int olmo355_attn_shared_prefix(const void* q, const void* kprefix, const void* vprefix, const void* kcache, const void* vcache,

@@ -53,3 +53,18 @@ def test_quantised_cache_and_shared_prefix_entries_refuse_without_launching():
                 dict(T=65), dict(Hkv=7), dict(bias=p, stride=63), dict(q=p + 4), dict(past=2**31 - 1)):
         assert prefix(**bad) == EINVAL, bad
     assert prefix(hd=48) == EUNSUP and prefix(dt=5) == EUNSUP and prefix(dev=p, T=2, wsb=2**40) == EUNSUP
+
+
+def test_a_workspace_for_n_keys_serves_fewer():
+    """The runs a call takes depend on its count of keys; the workspace of the largest count holds every smaller one's."""
+    from olmo_amd import _lib
+
+    h = _lib.lib()
+    for B, H, Hkv, hd in ((1, 32, 32, 128), (3, 40, 8, 128), (17, 8, 8, 64), (9, 32, 32, 32), (12, 32, 32, 128), (33, 8, 8, 64), (70, 48, 2, 32), (5, 8, 8, 128), (5, 1, 1, 128)):
+        sizes = [h.olmo355_attn_decode_q8_workspace_bytes(B, H, Hkv, hd, n) for n in (1, 127, 129, 2048, 2049, 2100, 4096, 100000)]
+        assert sizes == sorted(sizes), (B, H, Hkv, hd, sizes)
+        for T in (1, 3, 40, 250):
+            for dtype in (0, 1):
+                sizes = [h.olmo355_attn_shared_prefix_workspace_bytes(B, T, H, Hkv, hd, P, n, dtype)
+                         for P, n in ((1, 250), (100, 250), (129, 257), (129, 600), (1000, 1000), (2000, 1000), (2000, 5000), (60000, 5000), (60000, 9000))]
+                assert sizes == sorted(sizes), (B, T, H, Hkv, hd, dtype, sizes)
