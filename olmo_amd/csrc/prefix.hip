@@ -13,7 +13,7 @@ struct PrefixPlan {
   int rtp, rto;          // 16-row tiles per workgroup, prefix part and own part
   int tiles_p, tiles_o;  // row tiles per kv head (prefix) and per sequence and kv head (own)
   int splits_p, splits_o;
-  int most_p;              // splits_p for any fewer own keys (what a workspace has to hold)
+  int most;                // both for any fewer own or prefix keys (what a workspace has to hold)
   int64_t wgs_p, wgs_o;    // workgroups per kv head
   int64_t own_waves;       // waves of the own part per kv head
 };
@@ -27,14 +27,20 @@ PrefixPlan prefix_plan(int B, int T, int H, int Hkv, int P, int n_keys_max) {
   p.tiles_p = (int)((rows_p + 16 * p.rtp - 1) / (16 * p.rtp));
   p.tiles_o = (int)((rows_o + 16 * p.rto - 1) / (16 * p.rto));
   auto at_most = [](int64_t want, int64_t most) { return (int)(want < 1 ? 1 : want > most ? most : want); };
-  // Own keys: a wave per SIMD, at least two steps each.  Prefix: what fills the rest of two workgroups per CU, at least 128
-  // keys (a step per wave) each, so that the launch takes whole rounds: 4 sequences, 32 heads, prefix 16384 59 us with 512 +
-  // 32 workgroups, 52 with 480 + 32; 32 sequences, prefix 4001, 35-37 with 512 + 512 or 256 + 512, 33 with 256 + 256.
+  // Rounds of two workgroups per CU (512, or 2048 waves of own keys), shared between own keys and prefix in proportion to
+  // their keys, so that every wave has about as many: at least two steps of own keys each, a step per wave of the prefix's.
+  // Whole rounds matter more than the share: 32 heads, 8 sequences of 4000 own keys behind 1000 take 97 us with 448 + 64
+  // workgroups, 119 with 256 + 256, 129 with 256 + 32; 16 of 2000 behind 500 97 with 384 + 128, 126 with 256 + 128, 111 with
+  // 512 + 128; 4 under 16384 52 with 480 + 32, 59 with 512 + 32; 32 of 100 under 4001 29.5 with 256 + 256, 33 with 512 + 512.
+  // So own keys round down, and the prefix gets a round of its own only if what is left falls short of its share.
   // (The count of own keys is not looked at beyond that: a captured step is launched for as many as the cache holds.)
-  p.splits_o = at_most(1024 / ((int64_t)B * Hkv * p.tiles_o), (n_keys_max + 63ll) / 64);
+  const int64_t units_o = (int64_t)B * Hkv * p.tiles_o, units_p = (int64_t)Hkv * p.tiles_p;
+  const int64_t work_o = units_o * n_keys_max, work_p = units_p * P, steps_o = (n_keys_max + 63ll) / 64, steps_p = (P + 127ll) / 128;
+  const double share_p = (double)work_p / (double)(work_o + work_p);
+  p.splits_o = at_most((int64_t)(2048 * (1 - share_p)) / units_o, steps_o);
   const int64_t own = ((int64_t)B * p.tiles_o * p.splits_o + 3) / 4 * Hkv, room = 512 - own % 512;
-  p.splits_p = at_most((room < 192 ? room + 512 : room) / ((int64_t)Hkv * p.tiles_p), (P + 127ll) / 128);
-  p.most_p = at_most((192 + 511) / ((int64_t)Hkv * p.tiles_p), (P + 127ll) / 128);
+  p.splits_p = at_most((room < at_most((int64_t)(512 * share_p), 192) ? room + 512 : room) / units_p, steps_p);
+  p.most = at_most(2048 / units_o, steps_o) + at_most((192 + 511) / units_p, steps_p);
   p.wgs_p = (int64_t)p.tiles_p * p.splits_p;
   p.own_waves = (int64_t)B * p.tiles_o * p.splits_o;
   p.wgs_o = (p.own_waves + 3) / 4;
@@ -428,7 +434,7 @@ extern "C" int64_t olmo355_attn_shared_prefix_workspace_bytes(int B, int T, int 
   if (const int parts = prefix_chain_parts(B, T, H, Hkv, hd, prefix_len, n_keys_max, dtype))
     return parts == 1 ? 0 : 4 * rows_parts_floats((int64_t)B * T * H, hd, parts);
   const PrefixPlan p = prefix_plan(B, T, H, Hkv, prefix_len, n_keys_max);
-  return 4 * rows_parts_floats((int64_t)B * T * H, hd, p.most_p + p.splits_o);
+  return 4 * rows_parts_floats((int64_t)B * T * H, hd, p.most);
 }
 
 extern "C" int olmo355_attn_shared_prefix(const void* q, const void* kprefix, const void* vprefix, const void* kcache, const void* vcache,
