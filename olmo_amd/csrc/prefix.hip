@@ -13,12 +13,13 @@ struct PrefixPlan {
   int rtp, rto;          // 16-row tiles per workgroup, prefix part and own part
   int tiles_p, tiles_o;  // row tiles per kv head (prefix) and per sequence and kv head (own)
   int splits_p, splits_o;
-  int most;                // both for any fewer own or prefix keys (what a workspace has to hold)
+  int most;                // both for any fewer own or prefix keys, counted or not (what a workspace has to hold)
   int64_t wgs_p, wgs_o;    // workgroups per kv head
   int64_t own_waves;       // waves of the own part per kv head
 };
 
-PrefixPlan prefix_plan(int B, int T, int H, int Hkv, int P, int n_keys_max) {
+// counted: n_keys_max is the count of own keys, not a bound that a captured step was given.
+PrefixPlan prefix_plan(int B, int T, int H, int Hkv, int P, int n_keys_max, bool counted) {
   PrefixPlan p;
   const int64_t G = H / Hkv, rows_o = T * G, rows_p = B * rows_o;
   // (four tiles leave a SIMD one wave: 64 sequences of 32 heads under 2048 keys 66 us against 39, 256 sequences 175 against 114)
@@ -33,10 +34,11 @@ PrefixPlan prefix_plan(int B, int T, int H, int Hkv, int P, int n_keys_max) {
   // workgroups, 119 with 256 + 256, 129 with 256 + 32; 16 of 2000 behind 500 97 with 384 + 128, 126 with 256 + 128, 111 with
   // 512 + 128; 4 under 16384 52 with 480 + 32, 59 with 512 + 32; 32 of 100 under 4001 29.5 with 256 + 256, 33 with 512 + 512.
   // So own keys round down, and the prefix gets a round of its own only if what is left falls short of its share.
-  // (The count of own keys is not looked at beyond that: a captured step is launched for as many as the cache holds.)
+  // Where the count of own keys is only bounded, they get half a round: by proportion, 8 sequences of 50 keys out of 3000
+  // behind 1000 take 18 us instead of 12 (of 1900 51 instead of 61), 16 of 50 out of 2048, 8 kv heads, behind 2000 22 instead of 17.
   const int64_t units_o = (int64_t)B * Hkv * p.tiles_o, units_p = (int64_t)Hkv * p.tiles_p;
   const int64_t work_o = units_o * n_keys_max, work_p = units_p * P, steps_o = (n_keys_max + 63ll) / 64, steps_p = (P + 127ll) / 128;
-  const double share_p = (double)work_p / (double)(work_o + work_p);
+  const double share_p = counted ? (double)work_p / (double)(work_o + work_p) : 0.5;
   p.splits_o = at_most((int64_t)(2048 * (1 - share_p)) / units_o, steps_o);
   const int64_t own = ((int64_t)B * p.tiles_o * p.splits_o + 3) / 4 * Hkv, room = 512 - own % 512;
   p.splits_p = at_most((room < at_most((int64_t)(512 * share_p), 192) ? room + 512 : room) / units_p, steps_p);
@@ -433,7 +435,7 @@ extern "C" int64_t olmo355_attn_shared_prefix_workspace_bytes(int B, int T, int 
   if (!prefix_shape_ok(B, T, H, Hkv, prefix_len, n_keys_max) || hd <= 0) return 0;
   if (const int parts = prefix_chain_parts(B, T, H, Hkv, hd, prefix_len, n_keys_max, dtype))
     return parts == 1 ? 0 : 4 * rows_parts_floats((int64_t)B * T * H, hd, parts);
-  const PrefixPlan p = prefix_plan(B, T, H, Hkv, prefix_len, n_keys_max);
+  const PrefixPlan p = prefix_plan(B, T, H, Hkv, prefix_len, n_keys_max, true);
   return 4 * rows_parts_floats((int64_t)B * T * H, hd, p.most);
 }
 
@@ -463,7 +465,7 @@ extern "C" int olmo355_attn_shared_prefix(const void* q, const void* kprefix, co
     CHAIN(O355_F16, 64);
 #undef CHAIN
   }
-  const PrefixPlan plan = prefix_plan(B, T, H, Hkv, prefix_len, n_keys_max);
+  const PrefixPlan plan = prefix_plan(B, T, H, Hkv, prefix_len, n_keys_max, !past_len_dev && past_len + T == n_keys_max);
 #define PREFIX(DTv, HDv)                                                                                                           \
   return launch_shared_prefix<DTv, HDv>(q, kprefix, vprefix, kcache, vcache, key_bias, out, (float*)ws, B, T, H, Hkv, prefix_len,   \
                                         Pmax, Lmax, past_len, past_len_dev, n_keys_max, bias_stride, plan, as_stream(stream))
