@@ -469,7 +469,9 @@ class OLMo(nn.Module):
         prefix.  ``prefix_ids``: ``[P]`` or ``[1, P]``, at least one token."""
         if self.kv_cache is not None:
             raise NotImplementedError("a shared prefix is kept in the activation dtype: not with kv_cache='int8'")
-        ids = prefix_ids.view(1, -1)
+        if prefix_ids.dim() != 1 and (prefix_ids.dim() != 2 or prefix_ids.shape[0] != 1):
+            raise ValueError(f"one prompt expected, [P] or [1, P], not {tuple(prefix_ids.shape)}")
+        ids = prefix_ids.reshape(1, -1)
         P = ids.shape[1]
         if P < 1 or P >= self.max_cache_len:
             raise ValueError(f"a prefix of {P} tokens leaves no room in max_cache_len {self.max_cache_len}")
@@ -586,8 +588,6 @@ class OLMo(nn.Module):
             ws = self._prefix_ws(B, P, n_keys_max)
         else:
             ws = ops.attn_shared_prefix_workspace(B, T, H, Hkv, hd, P, n_keys_max, self.dtype, self.device)
-        if key_bias is not None and key_bias.shape[1] < n_keys_max:
-            key_bias = torch.nn.functional.pad(key_bias, (0, n_keys_max - key_bias.shape[1]))  # not visible: any value
         return ops.attn_shared_prefix(q, prefix.k[layer_id], prefix.v[layer_id], kc, vc, ws, B, T, H, Hkv, hd, P, past_len, n_keys_max,
                                       key_bias=key_bias, past_len_dev=graph_pos)
 
@@ -914,6 +914,8 @@ class OLMo(nn.Module):
         hidden: List[torch.Tensor] = []
         self._beam = cache if isinstance(cache, BeamKVCache) else None
         self._shared = cache.prefix if isinstance(cache, PrefixedKVCache) else None
+        if self._shared is not None and T == 1 and key_bias is not None and key_bias.shape[1] < cache.capacity:
+            key_bias = torch.nn.functional.pad(key_bias, (0, cache.capacity - key_bias.shape[1]))  # not visible: any value
         if self._beam is not None and T != 1:
             raise ValueError("a beam cache takes one token per row")
         decode = T == 1 and cache is not None and self._beam is None

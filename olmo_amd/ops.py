@@ -997,7 +997,7 @@ def _stream_of(dev: int) -> int:
 
 
 def _past_dev_ok(past_len_dev: Optional[torch.Tensor], T: int) -> None:
-    if past_len_dev is not None and (past_len_dev.dtype != torch.int32 or T != 1):
+    if past_len_dev is not None and (past_len_dev.dtype != torch.int32 or T != 1 or not past_len_dev.numel()):
         raise ValueError("past_len_dev: a device int32, for one token per sequence")
 
 
