@@ -221,7 +221,8 @@ __device__ __forceinline__ void walk_keys(const RowsIn& in, int step_lo, int ste
   const float* const bias = in.bias;
   const int lane = threadIdx.x & 63, col = lane & 15, kq = lane >> 4;
   const float c2 = kLog2e / sqrtf((float)HD);  // scores in the log2 domain
-  const float lowest = Act<DT>::lowest();
+  // the masked keys' score in the log2 domain; where it would pass fp32's range the type's own lowest is below all others too
+  const float lowest = DT == O355_F16 ? Act<DT>::lowest() * kLog2e : Act<DT>::lowest();
   auto& o = acc.o;
   auto& m = acc.m;
   auto& l = acc.l;

@@ -102,6 +102,22 @@ def test_cache_of_more_sequences_than_the_batch(dev):
     assert torch.equal(a, b) and torch.isfinite(a).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_heavy_penalty_is_not_a_mask(dev, dtype):
+    """The only key that is not masked carries a penalty near the end of fp16's range: its value comes out."""
+    ops = _ops()
+    B, H, Hkv, hd, keys = 2, 4, 2, 64, 200
+    cache, host = codes_case(dev, B, Hkv, keys, hd, seed=8)
+    q = torch.randn(B, 1, H * hd, generator=torch.Generator().manual_seed(9)).to(dtype)
+    bias = torch.full((B, keys), float("-inf"))
+    bias[0, 7], bias[1, 199] = -60000.0, -50000.0
+    ws = ops.attn_decode_q8_workspace(B, H, Hkv, hd, keys, dev)
+    out = ops.attn_decode_q8(q.to(dev), cache, ws, B, H, Hkv, hd, keys - 1, keys, key_bias=bias.to(dev)).cpu().double().view(B, Hkv, H // Hkv, hd)
+    for b, at in ((0, 7), (1, 199)):  # weight 1, exact; scale and result are rounded, in fp32 or to the type (or bf16, twice)
+        v = (host[1][b, :, at].double() * host[3][b, :, at, None].double())[:, None]
+        assert ((out[b] - v).abs() <= (2.0 ** -15 + torch.finfo(dtype).eps / 2) * v.abs() + 2.0 ** -25).all()
+
+
 def test_position_of_no_elements_is_refused(dev):
     ops = _ops()
     c = ops.KVQ8.empty(1, 2, 8, 64, dev)
