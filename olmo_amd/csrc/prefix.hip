@@ -229,8 +229,10 @@ __global__ __launch_bounds__(256, 2) void attn_prefix_chain_kernel(const uint16_
 #pragma unroll
   for (int ht = 0; ht < HT; ++ht) v_rd[ht] = (4 * kq + (col >> 2)) * VROW + ((ht ^ v_swz(4 * kq + (col >> 2))) << 5) + 8 * (col & 3);
 
-  fetch(first_tile, 0);
-  publish(0);
+  if (first_tile < tiles) {  // the first rows of a long prompt see fewer tiles than there are parts: such a part has no tile to ask for
+    fetch(first_tile, 0);
+    publish(0);
+  }
   int buf = 0;
   for (int tile = first_tile; tile < tiles; ++tile, buf ^= 1) {
     if (tile + 1 < tiles) fetch(tile + 1, buf ^ 1);  // read during the tile before, and everybody is past that tile's barrier

@@ -51,6 +51,17 @@ def test_launch_for_more_keys_than_there_are(dev, dtype, hd, T, past):
         assert ((out.cpu().double() - ref).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("B,T,P,past,H,Hkv,hd", [(1, 1000, 64, 0, 8, 1, 128), (1, 700, 1, 0, 3, 1, 64), (2, 520, 100, 1, 6, 2, 128)])
+def test_more_parts_than_the_first_rows_have_tiles(dev, B, T, P, past, H, Hkv, hd):
+    """A long prompt behind a short prefix: the keys are cut for the last rows, so the first rows' later parts are empty."""
+    args = (B, T, P, past, H, Hkv, hd)
+    print("empty parts", args, flush=True)
+    for dtype in (torch.bfloat16, torch.float16):
+        x = case(dtype, *args, seed=T)
+        ref, tol = reference(*x, *args)
+        assert ((call(dev, *x, *args).cpu().double() - ref).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("T", [3, 50])
 def test_captured_calls_of_several_tokens_and_two_streams(dev, T):
     """Both forms for several tokens replay, and two calls run at once on two streams, each with its workspace."""
