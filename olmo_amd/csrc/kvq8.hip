@@ -58,12 +58,12 @@ __device__ __forceinline__ void st8f(void* p, int64_t e, const float (&f)[8]) {
 }
 
 // ---- write ----------------------------------------------------------------------------------------------------
-// Grid (token rows, part): part 0 normalises and rotates q, part 1 k, part 2 takes v: the sum of squares of q and of k are
-// over the whole width (olmo/model.py:603-605), so whoever takes a part needs one of them and reads nothing twice.  A row's
-// part is one wave's (WPR 1: no barrier, four tokens to a workgroup) or a workgroup's (WPR 4).  A lane owns channels
-// j .. j + 7 of the first half of a head and the 8 they rotate with, CPT such pairs, which stay in registers as they were
-// loaded; hd / 16 neighbouring lanes hold a head, whose maximum is a few register exchanges.  fp32 from the input to the
-// code (q: to its one rounding).
+// Part 0 normalises and rotates q, part 1 k, part 2 takes v: the sum of squares of q and of k are over the whole width
+// (olmo/model.py:603-605), so whoever takes a part needs one of them and reads nothing twice.  A row's part is a workgroup's
+// (WPR 4; grid (token rows, part)) or q_lanes / kv_lanes lanes' of a wave (WPR 1: no barrier; a wave takes as many rows as
+// its 64 lanes hold; grid: part after part).  A lane owns channels j .. j + 7 of the first half of a head and the 8 they
+// rotate with, CPT such pairs, which stay in registers as they were loaded; hd / 16 neighbouring lanes hold a head, whose
+// maximum is a few register exchanges.  fp32 from the input to the code (q: to its one rounding).
 template <int DT, int HD, int CPT, int WPR>
 __global__ __launch_bounds__(256) void kv_write_q8_kernel(const void* __restrict__ qkv, const void* __restrict__ qw,
                                                           const void* __restrict__ kw, const float* __restrict__ sin_t,
@@ -71,12 +71,20 @@ __global__ __launch_bounds__(256) void kv_write_q8_kernel(const void* __restrict
                                                           int8_t* __restrict__ kq, int8_t* __restrict__ vq, float* __restrict__ ks,
                                                           float* __restrict__ vs, void* __restrict__ kc, void* __restrict__ vc, int Lfull,
                                                           uint32_t rows, uint32_t T, int H, int Hkv, int Lmax, int n_pos, int past_len,
-                                                          const int32_t* __restrict__ past_dev, float eps) {
+                                                          const int32_t* __restrict__ past_dev, float eps, int q_lanes, int kv_lanes,
+                                                          uint32_t q_blocks, uint32_t kv_blocks) {
   constexpr int CPH = HD / 16, HALF = HD / 2, LANES = 64 * WPR;
   __shared__ float red[16];
-  const int part = blockIdx.y, me = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
-  const uint32_t row = WPR == 1 ? blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x;
-  if (row >= rows) return;  // WPR 1: whole waves
+  int part = blockIdx.y, me = threadIdx.x, lanes = LANES;
+  uint32_t row = blockIdx.x;
+  if constexpr (WPR == 1) {
+    part = blockIdx.x < q_blocks ? 0 : blockIdx.x < q_blocks + kv_blocks ? 1 : 2;
+    lanes = part == 0 ? q_lanes : kv_lanes;  // a power of two; below 64 only where it holds the whole row
+    const uint32_t block = part == 0 ? blockIdx.x : blockIdx.x - q_blocks - (part - 1) * kv_blocks;
+    row = block * (256u / (uint32_t)lanes) + (uint32_t)threadIdx.x / (uint32_t)lanes;
+    me = threadIdx.x & (lanes - 1);
+  }
+  if (row >= rows) return;  // WPR 1: all lanes of a row
   const uint32_t b = row / T, t = row - b * T;
   const int dq = H * HD, dk = Hkv * HD;
   const int pos = (past_dev ? *past_dev : past_len) + (int)t;
@@ -105,8 +113,13 @@ __global__ __launch_bounds__(256) void kv_write_q8_kernel(const void* __restrict
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss += a[e] * a[e] + bb[e] * bb[e];
       }
-    if constexpr (WPR == 1) ss = wave_sum(ss);
-    else ss = block_sum(ss, red);
+    if constexpr (WPR == 1) {
+      if (lanes == 64) ss = wave_sum(ss);
+      else
+        for (int o = lanes >> 1; o; o >>= 1) ss += __shfl_xor(ss, o, 64);
+    } else {
+      ss = block_sum(ss, red);
+    }
     rstd = 1.f / sqrtf(ss / (float)(heads * HD) + eps);
   }
   const float* sn = sin_t + (int64_t)pos * HD;
@@ -298,13 +311,22 @@ extern "C" int olmo355_qknorm_rope_kvwrite_q8(const void* qkv, const void* qw, c
   hipStream_t s = as_stream(stream);
   const uint32_t rows = (uint32_t)B * T;
   // Few rows: a workgroup to a row's part, whose loads all go out at once (32 heads of 128, 1 row 4.8 us against 6.5 with a wave
-  // to it, 2048 rows 20.6 against 21.3); many rows, or short ones: a wave (40 heads, 8168 rows 95 against 97-104; 40 / 8
-  // heads, 8192 rows 52 against 59; 8 heads of 32, 8000 rows 15.5 against 25: the count of workgroups is what that costs).
+  // to it, 2048 rows 20.6 against 21.3); many rows: a wave (40 heads, 8168 rows 95 against 97-104; 40 / 8 heads, 8192 rows 52
+  // against 59), or as many lanes as the row has pairs: the count of waves is what short rows cost (8 heads of 32, 8000 rows
+  // 8.7 us against 15.7 with a wave and 25 with a workgroup to each; 16 / 2 heads of 64, 102032 rows 110 against 180).
   // 8168 rows of 40 heads: 4.4 TB/s of the 4.8 that a large copy reaches.
+  auto lanes_for = [hd](int heads) {
+    int n = 2;
+    while (n < 64 && n < heads * (hd / 16)) n *= 2;
+    return n;
+  };
+  const int q_lanes = lanes_for(H), kv_lanes = lanes_for(Hkv);
+  auto blocks_for = [rows](int lanes) { return (uint32_t)(((int64_t)rows * lanes + 255) / 256); };
+  const uint32_t q_blocks = blocks_for(q_lanes), kv_blocks = blocks_for(kv_lanes);
 #define WRITE(DTv, HDv, CPT, WPR)                                                                                                  \
-  hipLaunchKernelGGL((kv_write_q8_kernel<DTv, HDv, CPT, WPR>), dim3(WPR == 1 ? (rows + 3) / 4 : rows, 3), dim3(256), 0, s, qkv, qw, \
-                     kw, sin_tab, cos_tab, q_out, kq, vq, kscale, vscale, kcache, vcache, Lfull, rows, (uint32_t)T, H, Hkv, Lmax,   \
-                     n_pos, past_len, past_len_dev, eps)
+  hipLaunchKernelGGL((kv_write_q8_kernel<DTv, HDv, CPT, WPR>), WPR == 1 ? dim3(q_blocks + 2 * kv_blocks) : dim3(rows, 3), dim3(256), 0, \
+                     s, qkv, qw, kw, sin_tab, cos_tab, q_out, kq, vq, kscale, vscale, kcache, vcache, Lfull, rows, (uint32_t)T, H,    \
+                     Hkv, Lmax, n_pos, past_len, past_len_dev, eps, q_lanes, kv_lanes, q_blocks, kv_blocks)
 #define WRITE_CPT(DTv, HDv)                            \
   do {                                                 \
     if (rows < 4096 && chunks > 128) {                 \
