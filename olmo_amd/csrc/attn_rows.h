@@ -218,6 +218,10 @@ __device__ __forceinline__ void walk_keys(const RowsIn& in, int step_lo, int ste
   typedef Frag8<Keys::PV> FP;
   constexpr int STEPS = HD / 32, VC = HD / 16, ES = DT == O355_F32 ? 4 : 2;
   constexpr int KROW = Keys::SCALED ? HD : HD * ES;  // bytes of a key row
+  // fp32 heads of 128 under two row tiles: K and V of a step are 64 registers each beside 128 of q and o.  They take turns in
+  // the same 64 (V is asked for behind the first product, K behind the second), so that two waves fit a SIMD
+  // (41 sequences x 17 tokens of 32 / 16 heads behind 517 keys 136 -> 105 us; 64 x 1 of 8 heads behind 4001 39 -> 32).
+  constexpr bool TURNS = DT == O355_F32 && HD == 128 && RT == 2;
   const float* const bias = in.bias;
   const int lane = threadIdx.x & 63, col = lane & 15, kq = lane >> 4;
   const float c2 = kLog2e / sqrtf((float)HD);  // scores in the log2 domain
@@ -294,7 +298,8 @@ __device__ __forceinline__ void walk_keys(const RowsIn& in, int step_lo, int ste
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) s[rt][kt] = FQ::mma(kf, qf[rt][st], st == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[rt][kt]);
       }
-    if constexpr (MORE) request_k(step + stride);
+    if constexpr (TURNS) request_v(step);
+    else if constexpr (MORE) request_k(step + stride);
     if constexpr (Keys::SCALED) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -369,10 +374,11 @@ __device__ __forceinline__ void walk_keys(const RowsIn& in, int step_lo, int ste
         if constexpr (Keys::REST) o[rt][j] = FP::mma(vf, pl[rt], o[rt][j]);
       }
     }
-    if constexpr (MORE) request_v(step + stride);
+    if constexpr (MORE && TURNS) request_k(step + stride);
+    else if constexpr (MORE) request_v(step + stride);
   };
   request_k(step_lo);
-  request_v(step_lo);
+  if constexpr (!TURNS) request_v(step_lo);
   int step = step_lo;
   for (; step + stride < step_hi; step += stride) multiply(step, std::true_type{});
   multiply(step, std::false_type{});

@@ -49,8 +49,10 @@ PrefixPlan prefix_plan(int B, int T, int H, int Hkv, int P, int n_keys_max, bool
   return p;
 }
 
+// Two waves per SIMD in every instance: with the registers of one the compiler keeps accumulators and operands in AGPRs, and its
+// scheduler has then let scores overwrite value words that a product had still to read (fp32).
 template <int DT, int HD, int RTP, int RTO>
-__global__ __launch_bounds__(256, (DT != O355_F32 || HD < 128 ? 2 : 1)) void attn_shared_prefix_kernel(
+__global__ __launch_bounds__(256, 2) void attn_shared_prefix_kernel(
     const void* __restrict__ q, const void* __restrict__ kp, const void* __restrict__ vp, const void* __restrict__ kc,
     const void* __restrict__ vc, const float* __restrict__ key_bias, float* __restrict__ ws, int B, int T, int G, int Hkv, int P,
     int64_t Pmax, int64_t Lmax, int past_len, const int32_t* __restrict__ past_dev, int n_keys_max, int bias_stride, PrefixPlan plan) {
