@@ -175,8 +175,19 @@ __global__ __launch_bounds__(256) void kv_write_q8_kernel(const void* __restrict
     if constexpr (CPH >= 8) amax = fmaxf(amax, dpp_lane<0x141>(amax)); // row_half_mirror
     const bool ok = amax < INFINITY;
     const float scale = ok ? fmaxf(amax / 127.f, 1.1754943508222875e-38f) : __builtin_nanf("");
-    const float inv = ok ? 1.f / scale : 0.f;
-    auto code = [&](float v) { return ok ? (uint32_t)(uint8_t)(int8_t)(int)rintf(v * inv) : 0u; };
+    // v / scale, correctly rounded, with one division a row: two refinements of v * (1 / scale) by its residual (P. Markstein: a
+    // quotient within a unit of the last place, refined with the correctly rounded reciprocal and an exact residual, is the
+    // rounded quotient).  `up` keeps the residuals of rows of tiny values exact.  v * (1 / scale) alone moves codes next to a
+    // tie (a 16-bit value of half the row's maximum is at one); 8168 rows of 40 heads take 96 us with it, 103 so, 110 with a
+    // division per value.
+    const float up = scale < 0x1p-96f ? 0x1p96f : 1.f, s = scale * up, inv = 1.f / s;
+    auto code = [&](float v) {
+      v *= up;
+      float t = v * inv;
+      t = __builtin_fmaf(__builtin_fmaf(-t, s, v), inv, t);
+      t = __builtin_fmaf(__builtin_fmaf(-t, s, v), inv, t);
+      return ok ? (uint32_t)(uint8_t)(int8_t)(int)rintf(t) : 0u;
+    };
     u32x2 p1, p2;
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
@@ -310,11 +321,11 @@ extern "C" int olmo355_qknorm_rope_kvwrite_q8(const void* qkv, const void* qw, c
   if (chunks > 1024 || (int64_t)B * T > 0x7fffffff) return O355_EUNSUPPORTED;
   hipStream_t s = as_stream(stream);
   const uint32_t rows = (uint32_t)B * T;
-  // Few rows: a workgroup to a row's part, whose loads all go out at once (32 heads of 128, 1 row 4.8 us against 6.5 with a wave
-  // to it, 2048 rows 20.6 against 21.3); many rows: a wave (40 heads, 8168 rows 95 against 97-104; 40 / 8 heads, 8192 rows 52
-  // against 59), or as many lanes as the row has pairs: the count of waves is what short rows cost (8 heads of 32, 8000 rows
-  // 8.7 us against 15.7 with a wave and 25 with a workgroup to each; 16 / 2 heads of 64, 102032 rows 110 against 180).
-  // 8168 rows of 40 heads: 4.4 TB/s of the 4.8 that a large copy reaches.
+  // Few rows: a workgroup to a row's part, whose loads all go out at once (32 heads of 128, 1 row 4.0 us against 7.3 with a wave
+  // to it, 2048 rows 20.9 against 22.3); many rows: a wave (40 heads, 8168 rows 103 against 106; 40 / 8 heads, 8192 rows 53
+  // against 65), or as many lanes as the row has pairs: the count of waves is what short rows cost (8 heads of 32, 8000 rows
+  // 8.5 us against 18 with a wave and 35 with a workgroup to each; 16 / 2 heads of 64, 102032 rows 114 against 206 and 412).
+  // 8168 rows of 40 heads: 4.1 TB/s of the 4.8 that a large copy reaches.  (Replays of a graph of such calls.)
   auto lanes_for = [hd](int heads) {
     int n = 2;
     while (n < 64 && n < heads * (hd / 16)) n *= 2;
