@@ -171,6 +171,7 @@ __global__ __launch_bounds__(256, 2) void attn_prefix_chain_kernel(const uint16_
                                                                    int64_t Pmax, int64_t Lmax, int past, int bias_stride, int parts) {
   typedef Frag8<DT> F;
   constexpr int KT = 64, STEPS = HD / 32, HT = HD / 16, QT = 2, TILE = ChainLds<HD>::TILE, CPR = HD / 8, VROW = HD * 2;
+  constexpr bool REST = DT == O355_F16;
   extern __shared__ __align__(16) unsigned char smem[];
   unsigned char* const lds_k = smem;
   unsigned char* const lds_v = smem + 2 * TILE;
@@ -290,7 +291,9 @@ __global__ __launch_bounds__(256, 2) void attn_prefix_chain_kernel(const uint16_
             }
           }
       }
-      typename F::T pf[QT][2];
+      // fp16 weights keep 22 bits, as in attn_rows.h (olmo355_attn_prefill has them in fp32; 8 x 250 tokens, 32 heads, prefix 2048
+      // 110 us, 82 with weights of 11 bits); bf16 weights are rounded once (8 bits), as olmo355_attn_prefill has them
+      typename F::T pf[QT][2], pl[QT][2];
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
         float tmax = -INFINITY;
@@ -310,7 +313,7 @@ __global__ __launch_bounds__(256, 2) void attn_prefix_chain_kernel(const uint16_
             for (int r = 0; r < 4; ++r) o[qt][ht][r] *= alpha;
           m[qt] = mn;
         }
-        const float mref = m[qt] == -INFINITY ? 0.f : m[qt];  // a row that has seen no key yet
+        const float mref = (m[qt] == -INFINITY ? 0.f : m[qt]) - kWeightTop<DT>;  // 0: a row that has seen no key yet
         float p[4][4], psum = 0.f;
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt)
@@ -322,8 +325,13 @@ __global__ __launch_bounds__(256, 2) void attn_prefix_chain_kernel(const uint16_
         l[qt] += psum;
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2) {
-          const float f[8] = {p[2 * s2][0], p[2 * s2][1], p[2 * s2][2], p[2 * s2][3], p[2 * s2 + 1][0], p[2 * s2 + 1][1], p[2 * s2 + 1][2], p[2 * s2 + 1][3]};
+          float f[8] = {p[2 * s2][0], p[2 * s2][1], p[2 * s2][2], p[2 * s2][3], p[2 * s2 + 1][0], p[2 * s2 + 1][1], p[2 * s2 + 1][2], p[2 * s2 + 1][3]};
           pf[qt][s2] = F::pack(f);
+          if constexpr (REST) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = F::rest(f[i]);
+            pl[qt][s2] = F::pack(f);
+          }
         }
       }
       // ---- O^T += V^T . P^T
@@ -354,7 +362,10 @@ __global__ __launch_bounds__(256, 2) void attn_prefix_chain_kernel(const uint16_
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
-          for (int qt = 0; qt < QT; ++qt) o[qt][ht] = F::mma(__builtin_bit_cast(typename F::T, vf[ht][s2]), pf[qt][s2], o[qt][ht]);
+          for (int qt = 0; qt < QT; ++qt) {
+            o[qt][ht] = F::mma(__builtin_bit_cast(typename F::T, vf[ht][s2]), pf[qt][s2], o[qt][ht]);
+            if constexpr (REST) o[qt][ht] = F::mma(__builtin_bit_cast(typename F::T, vf[ht][s2]), pl[qt][s2], o[qt][ht]);
+          }
     }
     publish(buf ^ 1);  // the next tile is in LDS and this one has been read by everybody
   }
