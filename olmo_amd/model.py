@@ -560,12 +560,13 @@ class OLMo(nn.Module):
         return ops.attn_prefill(q, kc, vc, B, T, H, Hkv, hd, past_len, key_bias=key_bias)
 
     def _attention_q8(self, qkv, qw, kw, layer: ops.KVQ8, B, T, past_len, key_bias, graph_pos, n_keys_max):
-        """Attention over an 8-bit cache: one token per sequence reads the codes; several are attended to in the
-        activation dtype (earlier rows read back, the new ones as they are) while their codes are stored."""
+        """Attention over an 8-bit cache: a decode step (one token per sequence behind earlier ones) reads the codes; prompts
+        and several tokens are attended to in the activation dtype (earlier rows read back, the new ones as they are) while
+        their codes are stored."""
         c = self.config
         H, Hkv, hd = c.n_heads, c.effective_n_kv_heads, c.head_dim
         sin, cos = self._rope
-        if T == 1:
+        if T == 1 and (graph_pos is not None or past_len > 0):
             q = ops.qknorm_rope_kvwrite_q8(qkv, qw, kw, sin, cos, layer, B, T, H, Hkv, hd, past_len, c.layer_norm_eps,
                                            past_len_dev=graph_pos)
             return ops.attn_decode_q8(q, layer, self._q8_ws(B, n_keys_max), B, H, Hkv, hd, past_len, n_keys_max, key_bias=key_bias,
