@@ -130,6 +130,15 @@ class PrefixedKVCache(KVCache):
     def __init__(self, prefix: SharedPrefix, n_layers: int, B: int, Hkv: int, capacity: int, hd: int, dtype, device):
         super().__init__(n_layers, B, Hkv, capacity, hd, dtype, device)
         self.prefix = prefix
+        self._ws: Optional[torch.Tensor] = None
+
+    def decode_ws(self, n_heads: int) -> torch.Tensor:
+        """Workspace of the decode steps, the same from step to step (captured ones go on using it); it goes with the cache."""
+        if self._ws is None:
+            k = self.k[0]
+            self._ws = ops.attn_shared_prefix_workspace(self.B, 1, n_heads, k.shape[1], k.shape[3], self.prefix.length, self.capacity,
+                                                        k.dtype, k.device)
+        return self._ws
 
     def like(self, B: int) -> "PrefixedKVCache":
         k = self.k[0]
@@ -404,7 +413,7 @@ class OLMo(nn.Module):
         self._relay: Optional[_RelayState] = None  # state of the one-row decode relay, made on first use
         self._rope_now = None  # rotary rows of the current position during a captured decode step
         self._beam = None  # the beam cache while a beam-search step runs
-        self._shared: Optional[SharedPrefix] = None  # the prefix while tokens behind one run
+        self._shared: Optional[PrefixedKVCache] = None  # the cache while tokens behind a shared prefix run
         self._prepared = True
         return self
 
@@ -514,15 +523,6 @@ class OLMo(nn.Module):
             self._attn_ws[key] = ops.attn_decode_q8_workspace(B, c.n_heads, c.effective_n_kv_heads, c.head_dim, key[2], self.device)
         return self._attn_ws[key]
 
-    def _prefix_ws(self, B: int, P: int, n_keys_max: int) -> torch.Tensor:
-        """Workspace of a decode step behind a shared prefix, kept: captured steps go on using it."""
-        key = ("prefix", B, P, n_keys_max)
-        if key not in self._attn_ws:
-            c = self.config
-            self._attn_ws[key] = ops.attn_shared_prefix_workspace(B, 1, c.n_heads, c.effective_n_kv_heads, c.head_dim, P, n_keys_max,
-                                                                  self.dtype, self.device)
-        return self._attn_ws[key]
-
     # ------------------------------------------------------------------------------------------
     # one block: olmo/model.py:728-823 (wiring), :588-654 (attention)
     # ------------------------------------------------------------------------------------------
@@ -579,14 +579,14 @@ class OLMo(nn.Module):
 
     def _attention_shared(self, layer_id, qkv, qw, kw, kc, vc, B, T, past_len, key_bias, graph_pos, n_keys_max):
         """Attention behind a shared prefix: the own rows' positions follow the prefix's."""
-        c, prefix = self.config, self._shared
+        c, prefix = self.config, self._shared.prefix
         H, Hkv, hd, P = c.n_heads, c.effective_n_kv_heads, c.head_dim, prefix.length
         sin, cos = self._rope
         q = ops.qknorm_rope_kvwrite(qkv, qw, kw, sin[P:], cos[P:], kc, vc, B, T, H, Hkv, hd, past_len, c.layer_norm_eps,
                                     past_len_dev=graph_pos)
         if T == 1:  # one workspace and one split of the keys for every step, eager or captured
             n_keys_max = kc.shape[2]
-            ws = self._prefix_ws(B, P, n_keys_max)
+            ws = self._shared.decode_ws(H)
         else:
             ws = ops.attn_shared_prefix_workspace(B, T, H, Hkv, hd, P, n_keys_max, self.dtype, self.device)
         return ops.attn_shared_prefix(q, prefix.k[layer_id], prefix.v[layer_id], kc, vc, ws, B, T, H, Hkv, hd, P, past_len, n_keys_max,
@@ -914,7 +914,7 @@ class OLMo(nn.Module):
         self._rope_now = cache.rope_now if (cache is not None and graph_pos is not None) else None
         hidden: List[torch.Tensor] = []
         self._beam = cache if isinstance(cache, BeamKVCache) else None
-        self._shared = cache.prefix if isinstance(cache, PrefixedKVCache) else None
+        self._shared = cache if isinstance(cache, PrefixedKVCache) else None
         if self._shared is not None and T == 1 and key_bias is not None and key_bias.shape[1] < cache.capacity:
             key_bias = torch.nn.functional.pad(key_bias, (0, cache.capacity - key_bias.shape[1]))  # not visible: any value
         if self._beam is not None and T != 1:
@@ -941,6 +941,7 @@ class OLMo(nn.Module):
                 x, pend = self._block_decode_fused(blk, x, pend, kc, vc, B, past_len, key_bias, graph_pos, n_keys_max)
             else:
                 x = self._block(blk, x, kc, vc, B, T, past_len, key_bias, graph_pos, n_keys_max)
+        self._shared = None
         done = False
         if pend is not None:  # the last block's update has no following linear to ride on
             ln_f = self.transformer["ln_f"]

@@ -2,6 +2,9 @@
 
 Logits are compared relative to their own size: fp32 forms that compute the same numbers in another order of sums to
 ``F32`` of the largest logit (test_gpu_model_caches.py)."""
+import gc
+import weakref
+
 import pytest
 import torch
 
@@ -19,3 +22,28 @@ def test_int8_prompt_sees_its_own_rows_unrounded(dev, kind, T):  # noqa: F811
     a, b = q8(x, use_cache=True), plain(x, use_cache=True)
     assert close32(a.logits, b.logits)
     assert a.attn_key_values[0].cache.length == T
+
+
+def test_prefix_workspaces_go_with_their_caches(dev):  # noqa: F811
+    """Decode steps behind prefixes of many lengths leave nothing behind in the model: the workspace belongs to the sequences'
+    cache, is the same from step to step and is given back with it."""
+    m = build("gqa", torch.bfloat16, dev)
+    x = ids(4, 3, dev)
+
+    def steps(P):
+        out = m(x, use_cache=True, prefix=m.share_prefix(ids(1, P, dev)))
+        for _ in range(3):
+            out = m(x[:, :1], past_key_values=out.attn_key_values, use_cache=True)
+        cache = weakref.ref(out.attn_key_values[0].cache)
+        del out
+        gc.collect()
+        assert cache() is None
+        m.generate(x, max_steps=6, prefix=m.share_prefix(ids(1, P, dev)), stop_at_eos=False)
+
+    steps(50)
+    torch.cuda.synchronize()
+    kept, held = len(m._attn_ws), torch.cuda.memory_allocated()
+    for P in range(51, 75):
+        steps(P)
+    torch.cuda.synchronize()
+    assert len(m._attn_ws) == kept and torch.cuda.memory_allocated() <= held
