@@ -103,10 +103,18 @@ class QuantKVCache(KVCache):
         self.layers = [ops.KVQ8(codes[0, i], codes[1, i], scales[0, i], scales[1, i]) for i in range(n_layers)]
         self.k = [q.k for q in self.layers]
         self.v = [q.v for q in self.layers]
+        self._ws: Optional[torch.Tensor] = None
         self._books(B, capacity, device)
 
+    def decode_ws(self, n_heads: int) -> torch.Tensor:
+        """Workspace of the decode steps, for any count of keys up to the capacity; captured steps of two caches share none."""
+        if self._ws is None:
+            k = self.k[0]
+            self._ws = ops.attn_decode_q8_workspace(self.B, n_heads, k.shape[1], k.shape[3], self.capacity, k.device)
+        return self._ws
+
     def layer(self, i: int):
-        return self.layers[i], None
+        return self.layers[i], self
 
     def row_tensors(self) -> List[torch.Tensor]:
         return [t for q in self.layers for t in (q.k, q.v, q.k_scale, q.v_scale)]
@@ -515,14 +523,6 @@ class OLMo(nn.Module):
             self._attn_ws[key] = ops.attn_decode_workspace(B, c.n_heads, c.head_dim, key[1], self.device)
         return self._attn_ws[key]
 
-    def _q8_ws(self, B: int, n_keys_max: int) -> torch.Tensor:
-        """The same for the decode attention over an 8-bit cache."""
-        key = ("q8", B, -(-n_keys_max // 1024) * 1024)
-        if key not in self._attn_ws:
-            c = self.config
-            self._attn_ws[key] = ops.attn_decode_q8_workspace(B, c.n_heads, c.effective_n_kv_heads, c.head_dim, key[2], self.device)
-        return self._attn_ws[key]
-
     # ------------------------------------------------------------------------------------------
     # one block: olmo/model.py:728-823 (wiring), :588-654 (attention)
     # ------------------------------------------------------------------------------------------
@@ -536,7 +536,7 @@ class OLMo(nn.Module):
         qw = blk.q_norm.weight.data if blk.q_norm is not None else None
         kw = blk.k_norm.weight.data if blk.k_norm is not None else None
         if isinstance(kc, ops.KVQ8):
-            return self._attention_q8(qkv, qw, kw, kc, B, T, past_len, key_bias, graph_pos, n_keys_max)
+            return self._attention_q8(qkv, qw, kw, kc, vc, B, T, past_len, key_bias, graph_pos, n_keys_max)
         if self._shared is not None:
             return self._attention_shared(blk.layer_id, qkv, qw, kw, kc, vc, B, T, past_len, key_bias, graph_pos, n_keys_max)
         decode = T == 1 and (graph_pos is not None or past_len > 0)
@@ -559,7 +559,7 @@ class OLMo(nn.Module):
                                    key_bias=key_bias, past_len_dev=graph_pos)
         return ops.attn_prefill(q, kc, vc, B, T, H, Hkv, hd, past_len, key_bias=key_bias)
 
-    def _attention_q8(self, qkv, qw, kw, layer: ops.KVQ8, B, T, past_len, key_bias, graph_pos, n_keys_max):
+    def _attention_q8(self, qkv, qw, kw, layer: ops.KVQ8, cache: QuantKVCache, B, T, past_len, key_bias, graph_pos, n_keys_max):
         """Attention over an 8-bit cache: a decode step (one token per sequence behind earlier ones) reads the codes; prompts
         and several tokens are attended to in the activation dtype (earlier rows read back, the new ones as they are) while
         their codes are stored."""
@@ -569,7 +569,7 @@ class OLMo(nn.Module):
         if T == 1 and (graph_pos is not None or past_len > 0):
             q = ops.qknorm_rope_kvwrite_q8(qkv, qw, kw, sin, cos, layer, B, T, H, Hkv, hd, past_len, c.layer_norm_eps,
                                            past_len_dev=graph_pos)
-            return ops.attn_decode_q8(q, layer, self._q8_ws(B, n_keys_max), B, H, Hkv, hd, past_len, n_keys_max, key_bias=key_bias,
+            return ops.attn_decode_q8(q, layer, cache.decode_ws(H), B, H, Hkv, hd, past_len, n_keys_max, key_bias=key_bias,
                                       past_len_dev=graph_pos)
         kc, vc = self._scratch_cache(B, past_len + T)
         if past_len:

@@ -47,3 +47,30 @@ def test_prefix_workspaces_go_with_their_caches(dev):  # noqa: F811
         steps(P)
     torch.cuda.synchronize()
     assert len(m._attn_ws) == kept and torch.cuda.memory_allocated() <= held
+
+
+@pytest.mark.parametrize("form", ["int8", "prefix"])
+def test_sessions_of_two_caches_share_no_workspace(dev, form, monkeypatch):  # noqa: F811
+    """What the attention of one session's captured steps writes while it runs is not another session's.  (Read from the calls'
+    arguments: a race between two streams shows only now and then.)"""
+    from olmo_amd import ops
+    from olmo_amd.generate import DecodeSession
+
+    name = "attn_decode_q8" if form == "int8" else "attn_shared_prefix"
+    call, at, used = getattr(ops, name), 2 if form == "int8" else 5, []
+    monkeypatch.setattr(ops, name, lambda *a, **k: (used.append((a[at].data_ptr(), a[at].numel())), call(*a, **k))[1])
+    m = build("gqa", torch.bfloat16, dev, kv_cache="int8" if form == "int8" else None)
+    prefix = None if form == "int8" else m.share_prefix(ids(1, 40, dev))
+    sessions = []
+    for i in range(2):
+        out = m(ids(2, 130, dev, seed=i), use_cache=True, last_logits_only=True, prefix=prefix)
+        sessions.append(DecodeSession(m, out.attn_key_values[0].cache, out.logits.argmax(-1), None))
+    ranges = []
+    for s in sessions:
+        used.clear()
+        s.step()
+        s.capture()
+        assert len(set(used)) == 1 and used[0][1] > 0
+        ranges.append(used[0])
+    (a, n), (b, m) = sorted(ranges)
+    assert a + 4 * n <= b
