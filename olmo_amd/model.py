@@ -492,9 +492,12 @@ class OLMo(nn.Module):
         P = ids.shape[1]
         if P < 1 or P >= self.max_cache_len:
             raise ValueError(f"a prefix of {P} tokens leaves no room in max_cache_len {self.max_cache_len}")
-        cache = self(ids, use_cache=True, last_logits_only=True).attn_key_values[0].cache
+        if not self._prepared:
+            self.post_init()
+        cache = self.new_cache(1, P)  # as long as the prompt: the prefix is the cache, nothing is copied or held besides
+        self._forward_tokens(self.transformer["wte"](ids.to(self.device)), cache, 1, P, 0, None, None, True)
         ops.streamk_check()
-        return SharedPrefix([k[0, :, :P].contiguous() for k in cache.k], [v[0, :, :P].contiguous() for v in cache.v], P)
+        return SharedPrefix([k[0] for k in cache.k], [v[0] for v in cache.v], P)
 
     def _prefixed_cache(self, prefix: SharedPrefix, B: int) -> PrefixedKVCache:
         c = self.config

@@ -74,3 +74,23 @@ def test_sessions_of_two_caches_share_no_workspace(dev, form, monkeypatch):  # n
         ranges.append(used[0])
     (a, n), (b, m) = sorted(ranges)
     assert a + 4 * n <= b
+
+
+@pytest.mark.parametrize("kind,Hkv", [("gqa", 2), ("mqa", 1)])
+def test_a_prefix_holds_its_own_rows_alone(dev, kind, Hkv):  # noqa: F811
+    """Whatever the count of kv heads: the memory behind a prefix is its rows', not that of a cache of the model's length."""
+    from olmo_amd.model import OLMo
+
+    from .test_gpu_model_caches import cfg
+
+    c = cfg("gqa")
+    c.n_kv_heads = Hkv
+    m = OLMo(c, device=dev, dtype=torch.bfloat16, max_cache_len=256)
+    m.reset_parameters(seed=3)
+    x = ids(1, 37, dev, seed=5)
+    p = m.share_prefix(x[0])  # (on a model that has not run yet)
+    storages = {t.untyped_storage().data_ptr(): t.untyped_storage().nbytes() for t in (*p.k, *p.v)}
+    assert sum(storages.values()) == sum(t.numel() * t.element_size() for t in (*p.k, *p.v)) == 2 * 3 * Hkv * 37 * 64 * 2
+    want = m(x, use_cache=True).attn_key_values
+    for i, (k, v) in enumerate(want):
+        assert torch.equal(p.k[i], k[0]) and torch.equal(p.v[i], v[0])
