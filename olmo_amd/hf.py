@@ -28,7 +28,7 @@ import torch.nn as nn
 
 from .config import ModelConfig
 from .generate import greedy_generate
-from .model import KVCache, LayerKV, OLMo
+from .model import KVCache, LayerKV, OLMo, PrefixedKVCache
 
 try:  # the HF surface proper needs transformers; everything else of the package does not
     from transformers import AutoConfig, AutoModelForCausalLM, GenerationMixin, PretrainedConfig, PreTrainedModel
@@ -274,12 +274,14 @@ class OLMoForCausalLM(*_ModelBase):
             raise ValueError("output_attentions is not yet supported in OLMo")  # modeling_olmo.py:103-104
         return_dict = return_dict if return_dict is not None else self.config.return_dict
 
-        # a transformers Cache: ours carries the buffers; an empty one means "no past"; a populated foreign one
-        # holds plain (k, v) per layer in the reference's form (keys not rotated) and is taken over as such
+        # a transformers Cache: ours carries the buffers; an empty one means "no past" (behind a shared prefix: no rows of
+        # its own, the prefix stays); a populated foreign one holds plain (k, v) per layer in the reference's form (keys
+        # not rotated) and is taken over as such
         cache_in = past_key_values if _is_cache_object(past_key_values) else None
         if cache_in is not None:
             if isinstance(cache_in, OLMoCache):
-                past_key_values = cache_in.legacy() if cache_in.kv.length > 0 else None
+                kept = cache_in.kv.length > 0 or isinstance(cache_in.kv, PrefixedKVCache)
+                past_key_values = cache_in.legacy() if kept else None
             elif cache_in.get_seq_length() == 0:
                 past_key_values = None
             else:

@@ -94,3 +94,22 @@ def test_a_prefix_holds_its_own_rows_alone(dev, kind, Hkv):  # noqa: F811
     want = m(x, use_cache=True).attn_key_values
     for i, (k, v) in enumerate(want):
         assert torch.equal(p.k[i], k[0]) and torch.equal(p.v[i], v[0])
+
+
+def test_transformers_cache_emptied_behind_a_prefix_keeps_the_prefix(dev):  # noqa: F811
+    """``crop`` and ``reset`` take back the sequences' own rows; the prefix is no row of theirs."""
+    from olmo_amd.hf import HAVE_TRANSFORMERS, OLMoCache, OLMoConfig, OLMoForCausalLM
+
+    if not HAVE_TRANSFORMERS:
+        pytest.skip("transformers is not installed")
+    m = build("gqa", torch.float32, dev)
+    hf = OLMoForCausalLM(OLMoConfig.from_model_config(m.config, use_cache=True), model=m)
+    prefix, x, y = m.share_prefix(ids(1, 40, dev)), ids(2, 9, dev, seed=1), ids(2, 5, dev, seed=2)
+    want = m(y, prefix=prefix).logits
+    c = OLMoCache(m(x, use_cache=True, prefix=prefix).attn_key_values[0].cache)
+    for empty in (lambda: c.crop(-9), c.reset):
+        empty()
+        assert c.get_seq_length() == 0
+        out = hf(y, past_key_values=c, use_cache=True)
+        assert torch.equal(out.logits, want)
+        assert out.past_key_values is c and c.get_seq_length() == 5 and c.kv.prefix is prefix
