@@ -395,13 +395,15 @@ __global__ __launch_bounds__(256, 2) void attn_prefix_chain_kernel(const uint16_
 }
 
 // Which form a call takes: the one-pass form where a sequence has rows to fill a good part of a workgroup's 128; the split
-// form (any type, head size and count of rows) elsewhere.  Measured, 32 heads of 128, prefix 2048, us split / one pass:
-// 8 x 16 tokens 49 / 54, 32 x 16 93 / 134, 8 x 32 62 / 54, 16 x 32 114 / 74, 8 x 64 89 / 55, 16 x 100 behind 100 keys 104 / 19.
+// form (any type, head size and count of rows) elsewhere.  Measured, 32 heads of 128, prefix 2048, us split / one pass, bf16:
+// 8 x 16 tokens 31 / 47, 32 x 16 81 / 150, 8 x 32 62 / 48, 16 x 32 77 / 77, 8 x 64 76 / 53, 16 x 100 behind 100 keys 66 / 19.
+// fp16, whose one-pass form has a second product: 16 x 32 78 / 108, 16 x 48 95 / 110, 4 x 56 35 / 41, 8 x 64 76 / 69,
+// 16 x 64 121 / 110, 16 x 100 behind 100 keys 66 / 22.
 // Parts: with fewer workgroups than two per CU the keys are shared too, at least four tiles of 64 to a workgroup
 // (eight: 1 x 64 tokens 23.3 us against 19.7, 2 x 40 tokens behind 517 keys 20.2 against 16.6).
 int prefix_chain_parts(int B, int T, int H, int Hkv, int hd, int P, int n_keys_max, int dtype) {
   const int64_t rows = (int64_t)T * (H / Hkv), blocks = (rows + 127) / 128, wgs = blocks * B * Hkv;
-  if (dtype == O355_F32 || hd == 32 || T == 1 || rows < 32) return 0;
+  if (dtype == O355_F32 || hd == 32 || T == 1 || rows < (dtype == O355_F16 ? 64 : 32)) return 0;
   const int64_t most = ((P + 63ll) / 64 + (n_keys_max + 63ll) / 64) / 4, want = 512 / wgs;
   const int64_t parts = want < 1 || most < 1 ? 1 : want > most ? most : want;
   return B <= 65535 && Hkv <= 65535 && blocks * parts <= 65535 ? (int)parts : 0;  // grid limits

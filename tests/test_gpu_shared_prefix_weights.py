@@ -66,7 +66,8 @@ def test_weights_are_not_rounded_to_the_type(dev, dtype, B, T, P, past, H, Hkv, 
     assert ((out.cpu().double() - ref).abs() <= tol).all()
 
 
-@pytest.mark.parametrize("B,T,P,past,H,Hkv,hd", [(1, 33, 6, 1, 1, 1, 64), (2, 40, 64, 3, 2, 2, 128), (3, 130, 30, 0, 4, 2, 128)])
+@pytest.mark.parametrize("B,T,P,past,H,Hkv,hd", [(1, 33, 6, 1, 1, 1, 64), (2, 40, 64, 3, 2, 2, 128), (3, 130, 30, 0, 4, 2, 128), (1, 65, 6, 1, 1, 1, 64),
+                                                 (2, 80, 64, 3, 2, 2, 128)])
 def test_fp16_weights_of_prompts(dev, B, T, P, past, H, Hkv, hd):  # noqa: F811
     """The one-pass form for prompts keeps them too in fp16 (bf16 prompts have weights of 8 bits, as ``attn_prefill``)."""
     print("prefix weights, prompt", B, T, P, past, H, Hkv, hd, flush=True)
