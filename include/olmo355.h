@@ -335,7 +335,9 @@ int olmo355_attn_decode_q8(const void* q, const int8_t* kq, const int8_t* vq, co
  * olmo355_attn_prefill / olmo355_attn_decode over a cache that begins with a copy of the prefix, read once for all sequences.
  * key_bias (may be NULL): fp32 [B, bias_stride] for the own rows; a masked one (<= -1e30) weighs nothing, whatever it
  * holds (the prefix is never masked, so no query is left without a key); a row that only causality hides from some of the
- * call's queries (T > 1) holds finite values, as in olmo355_attn_prefill.  prefix_len >= 1, n_keys_max >= T bounds the own
+ * call's queries (T > 1) holds finite values, as in olmo355_attn_prefill, and an infinite value that is seen makes the result
+ * NaN (16-bit weights are multiplied in two parts; bf16 prompts, whose weights are rounded once as in olmo355_attn_prefill,
+ * excepted).  prefix_len >= 1, n_keys_max >= T bounds the own
  * rows for the launch grid (past_len + T <= n_keys_max <= Lmax; fastest where it is their count); past_len_dev needs T == 1.  hd 32, 64 or 128; q, caches
  * and out 16-byte aligned.  ws as for olmo355_attn_decode_q8. */
 int64_t olmo355_attn_shared_prefix_workspace_bytes(int B, int T, int H, int Hkv, int hd, int prefix_len, int n_keys_max,

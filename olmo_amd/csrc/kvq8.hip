@@ -272,9 +272,11 @@ __global__ __launch_bounds__(256, 2) void attn_decode_q8_kernel(const void* __re
 // Runs of keys per (sequence, kv head, row tile), at least 128 keys each (one step per wave). A round of one workgroup per CU,
 // no more, is best where it keeps the CUs busy: 4 x 4096 keys, 32 heads, 28.8 us with 256 workgroups, 29.4 with 512;
 // 1 x 4096 12.4 against 13.0; 8 x 2048 26.0 against 29.0; 32 x 1000, 8 kv heads, 13.9 against 17.6 (one run each, no merge).
-// Where the last round would leave a quarter of the CUs idle, long keys are cut finer: 9 x 4096, 32 heads, 74.6 us in
-// whole runs, 63.1 in 3; 13 x 8000, 10 kv heads, 72 in whole runs, 57 in 3. Up to 2048 keys that costs more than it brings
-// (5 x 2000, 32 heads, 19.0 in whole runs, 20.2 in 3). Never less with more keys: a workspace for n serves fewer.
+// Where the last round would leave a quarter of the CUs idle, long keys are cut finer, into as many runs as four workgroups per
+// CU take: 9 x 4096, 32 heads, 74.8 us in whole runs, 63.6 in 3; 13 x 8000, 10 kv heads, 72 in whole runs, 58 in 3, 55 in the 7
+// it takes. Up to 2048 keys that would cost more than it brings (5 x 2000, 32 heads, 19.0 in whole runs, 20.2 in 3). So beyond
+// 128 (sequence, kv head, row tile) units keys stay whole, but for more than 2048 keys of 129-192 or 257-384 units.
+// Never fewer runs with more keys: a workspace for n serves fewer.
 int decode_q8_splits(int B, int H, int Hkv, int n_keys_max) {
   const int64_t units = (int64_t)B * Hkv * ((H / Hkv + 15) / 16), cus = 256;
   const int64_t whole = units < cus ? cus / units : 1, rounds = (units * whole + cus - 1) / cus;

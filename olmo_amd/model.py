@@ -587,7 +587,8 @@ class OLMo(nn.Module):
         sin, cos = self._rope
         q = ops.qknorm_rope_kvwrite(qkv, qw, kw, sin[P:], cos[P:], kc, vc, B, T, H, Hkv, hd, past_len, c.layer_norm_eps,
                                     past_len_dev=graph_pos)
-        if T == 1:  # one workspace and one split of the keys for every step, eager or captured
+        if T == 1:  # one workspace and one split of the keys for every step, eager or captured (the eager step that fills the
+            # cache alone has one of its own: there the bound is the count)
             n_keys_max = kc.shape[2]
             ws = self._shared.decode_ws(H)
         else:
@@ -994,7 +995,8 @@ class OLMo(nn.Module):
         over a :class:`BeamKVCache`.  ``scores`` is the
         summed log-probability of the chosen tokens under the unfiltered distribution (passed through
         ``final_sequence_scorer`` in a beam search).  ``prefix``: a prompt shared by the batch (:meth:`share_prefix`;
-        ``input_ids`` are what follows it), beam size 1 only."""
+        ``input_ids`` are what follows it), beam size 1 only; a sampler's draws count positions behind the prefix, so the same
+        prompt given whole draws other tokens."""
         if attention_bias is not None:  # olmo/model.py:1645-1657
             B, P = input_ids.shape
             assert attention_bias.dim() == 4 and tuple(attention_bias.shape[:2]) == (B, 1)
