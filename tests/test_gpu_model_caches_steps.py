@@ -220,3 +220,30 @@ def test_loaders_take_the_form_of_the_cache(dev, tmp_path):  # noqa: F811
     loaded = load_unsharded_checkpoint(str(d), device=str(dev), dtype=torch.float32, max_cache_len=256, kv_cache="int8")
     for a, b in zip(steps(loaded), steps(m)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind,dtype,B", MODELS)
+def test_prompts_of_one_token(dev, monkeypatch, kind, dtype, B):  # noqa: F811
+    """The shortest conversation: one token, then steps behind it, eager and captured, over codes and behind a prefix that fills
+    the model's length but for what follows."""
+    from olmo_amd.generate import greedy_generate
+
+    print("one token", kind, dtype, B, flush=True)
+    q8, plain = make(kind, dtype, dev, kv_cache="int8"), make(kind, dtype, dev)
+    x = ids(B, 1, dev, seed=B)
+    a, b = q8(x, use_cache=True), plain(x, use_cache=True)
+    assert near(a.logits, b.logits, dtype)
+    toks, logits = greedy_generate(q8, x, None, 6, return_logits=True)
+    assert torch.equal(logits[:, 0], a.logits[:, 0])
+    round_cache(b.attn_key_values[0].cache)
+    for t in range(5):
+        with rows_rounded(monkeypatch):
+            b = plain(toks[:, t:t + 1], past_key_values=b.attn_key_values, use_cache=True)
+        assert near(logits[:, t + 1], b.logits[:, 0], dtype)
+    head = ids(1, 250, dev, seed=7)  # 250 + 1 + 5: all 256 positions
+    prefix = plain.share_prefix(head)
+    toks, logits = greedy_generate(plain, x, None, 6, return_logits=True, prefix=prefix)
+    whole = plain(torch.cat((head.expand(B, 250), x, toks[:, :-1]), 1)).logits[:, 250:]
+    assert near(logits, whole, dtype)
+    with pytest.raises(ValueError):
+        greedy_generate(plain, x, None, 8, prefix=prefix)
